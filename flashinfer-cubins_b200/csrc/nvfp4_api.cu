@@ -23,6 +23,7 @@
 #include "nvfp4_gemm_kernel.cuh"
 #include "nvfp4_gemm_pair_kernel.cuh"
 #include "nvfp4_glue_kernels.cuh"
+#include "nvfp4_host.h"
 
 using namespace nvfp4;
 
@@ -71,10 +72,7 @@ struct DeviceGuard {
   }
 };
 
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
-                                   const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
-                                   const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+using EncodeTiledFn = EncodeTiled;
 
 // cuTensorMapEncodeTiled, looked up through the runtime so that the library has no
 // link-time dependency on libcuda (it must load on machines without a driver).
@@ -821,6 +819,19 @@ int create_dense_like(nvfp4_plan** out, int kind, int device, int out_kind, int 
 }
 
 }  // namespace
+
+// What the other translation units of the library use of this one (nvfp4_host.h).
+namespace nvfp4 {
+
+int host_fail(int code, const char* text) noexcept { return fail(code, "%s", text); }
+
+int host_fail_cuda(cudaError_t error, const char* what) noexcept { return fail_cuda(error, what); }
+
+int host_encoder(EncodeTiled* out) noexcept { return get_encoder(out); }
+
+int host_sm_count() noexcept { return current_sm_count(); }
+
+}  // namespace nvfp4
 
 extern "C" {
 
@@ -1799,6 +1810,17 @@ int nvfp4_moe_place_routed(const void* ids, int ids_are_64bit, long long pairs, 
   return moe_place_common(ids, ids_are_64bit, pairs, choices,
                           static_cast<int>(plan->problems.size()), nullptr, header->first_rows,
                           plan->routed_rows, cursors, row_of_pair, token_of_row, stream);
+}
+
+int nvfp4_moe_place_offsets(const void* ids, int ids_are_64bit, long long pairs, int choices,
+                            int experts, const int* offsets, int rows, int* cursors,
+                            int* row_of_pair, int* token_of_row, void* stream) {
+  if (offsets == nullptr) return fail(NVFP4_E_INVALID_ARGUMENT, "null operand");
+  if (pairs > rows) {
+    return fail(NVFP4_E_INVALID_ARGUMENT, "%lld pairs do not fit in %d rows", pairs, rows);
+  }
+  return moe_place_common(ids, ids_are_64bit, pairs, choices, experts, nullptr, offsets, rows,
+                          cursors, row_of_pair, token_of_row, stream);
 }
 
 int nvfp4_moe_combine(const void* y, const int* row_of_pair, const float* weights, float* out,

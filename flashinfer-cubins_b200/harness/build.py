@@ -13,8 +13,10 @@ import sys
 from pathlib import Path
 
 PACKAGE_ROOT = Path(__file__).resolve().parents[1]
-SOURCES = (PACKAGE_ROOT / "csrc" / "nvfp4_api.cu",)
-HEADERS = tuple(sorted((PACKAGE_ROOT / "csrc").glob("*.cuh"))) + (
+SOURCES = tuple(PACKAGE_ROOT / "csrc" / name for name in ("nvfp4_api.cu", "int8_api.cu"))
+HEADERS = (
+    *sorted((PACKAGE_ROOT / "csrc").glob("*.cuh")),
+    PACKAGE_ROOT / "csrc" / "nvfp4_host.h",
     PACKAGE_ROOT.parent / "include" / "nvfp4_b200.h",
 )
 OUTPUT = PACKAGE_ROOT / "lib" / "libnvfp4_b200.so"
@@ -23,6 +25,7 @@ FLAGS = (
     "-lineinfo", "-O3", "-std=c++17",
     "-shared", "-Xcompiler", "-fPIC",
     "-cudart", "static",
+    "-t", "2",  # the sources side by side
 )
 
 

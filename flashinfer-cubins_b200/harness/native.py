@@ -155,6 +155,28 @@ _PROTOTYPES = {
     "nvfp4_moe_combine": (
         ctypes.c_int, [_P, _P, _P, _P, ctypes.c_int, ctypes.c_int, ctypes.c_int, _P],
     ),
+    "nvfp4_moe_offsets": (ctypes.c_int, [_P, ctypes.c_int, _P, _P]),
+    "nvfp4_moe_place_offsets": (
+        ctypes.c_int, [_P, ctypes.c_int, ctypes.c_longlong, ctypes.c_int, ctypes.c_int, _P,
+                       ctypes.c_int, _P, _P, _P, _P],
+    ),
+    "nvfp4_int8_gemm": (
+        ctypes.c_int, [_P, ctypes.c_longlong, _P, ctypes.c_longlong, _P, _P, _P, _P,
+                       ctypes.c_longlong] + [ctypes.c_int] * 5 + [_P],
+    ),
+    "nvfp4_int8_group_gemm": (
+        ctypes.c_int, [_P, ctypes.c_longlong, _P, ctypes.c_longlong, ctypes.c_longlong, _P, _P, _P,
+                       _P, ctypes.c_longlong] + [ctypes.c_int] * 6 + [_P],
+    ),
+    "nvfp4_int8_quantize": (
+        ctypes.c_int, [_P, ctypes.c_int, ctypes.c_longlong, _P, ctypes.c_int, ctypes.c_int,
+                       ctypes.c_int, _P, ctypes.c_longlong, _P, _P],
+    ),
+    "nvfp4_residual_norm": (
+        ctypes.c_int, [_P, ctypes.c_int, ctypes.c_longlong, _P, ctypes.c_int, ctypes.c_longlong, _P,
+                       _P, ctypes.c_int, ctypes.c_float, _P, ctypes.c_double, _P, ctypes.c_longlong,
+                       _P, ctypes.c_int, ctypes.c_longlong, _P, ctypes.c_int, ctypes.c_int, _P],
+    ),
     "nvfp4_silu_product": (ctypes.c_int, [_P, _P, _P, ctypes.c_int64, _P]),
     "nvfp4_measure_mma_peak": (ctypes.c_int, [ctypes.c_int, ctypes.c_int, ctypes.POINTER(ctypes.c_double)]),
 }
@@ -411,6 +433,8 @@ def pack_scales(scales: int, packed: int, rows: int, cols: int, batches: int, st
 
 IN_F32 = 0
 IN_BF16 = 1
+IN_F16 = 2
+NORM_CODES = -1
 
 
 def quantize(x: int, x_kind: int, packed: int, scales: int, rows: int, k: int, batches: int,
@@ -444,6 +468,19 @@ def moe_place(ids: int, ids_are_64bit: bool, pairs: int, choices: int, first_row
     starts = (ctypes.c_int * len(first_rows))(*first_rows)
     check(load().nvfp4_moe_place(ids, int(ids_are_64bit), pairs, choices, len(first_rows), starts,
                                  rows, cursors, row_of_pair, token_of_row, stream))
+
+
+def moe_offsets(counts: int, experts: int, offsets: int, stream: int) -> None:
+    """``offsets[e]`` (device int32, ``experts + 1``) = pairs of the experts before e."""
+    check(load().nvfp4_moe_offsets(counts, experts, offsets, stream))
+
+
+def moe_place_offsets(ids: int, ids_are_64bit: bool, pairs: int, choices: int, experts: int,
+                      offsets: int, rows: int, cursors: int, row_of_pair: int, token_of_row: int,
+                      stream: int) -> None:
+    """``moe_place`` with the experts' first rows on the device, unpadded."""
+    check(load().nvfp4_moe_place_offsets(ids, int(ids_are_64bit), pairs, choices, experts, offsets,
+                                         rows, cursors, row_of_pair, token_of_row, stream))
 
 
 def moe_combine(y: int, row_of_pair: int, weights: int, out: int, tokens: int, choices: int,

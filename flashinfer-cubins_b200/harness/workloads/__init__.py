@@ -1,3 +1,3 @@
-"""Importing this package registers the NVFP4 workloads."""
+"""Importing this package registers the NVFP4 and INT8 workloads."""
 
-from . import nvfp4_dual_gemm, nvfp4_gemm, nvfp4_group_gemm  # noqa: F401
+from . import int8, nvfp4_dual_gemm, nvfp4_gemm, nvfp4_group_gemm  # noqa: F401

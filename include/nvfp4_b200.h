@@ -267,6 +267,7 @@ int nvfp4_pack_scales(const void* scales, void* packed, int rows, int cols, int 
 /* Input kinds of nvfp4_quantize. */
 #define NVFP4_IN_F32 0
 #define NVFP4_IN_BF16 1
+#define NVFP4_IN_F16 2 /* the 8-bit-integer operators only */
 
 /* FP32 or BF16 x[batches][rows][k] -> NVFP4: packed E2M1 [batches][rows][k/2] and UE4M3
  * scales written straight into the blocked layout (zero padded). Per 16-element K block
@@ -353,6 +354,65 @@ int nvfp4_moe_place_routed(const void* ids, int ids_are_64bit, long long pairs, 
  * nothing). hidden % 8 == 0; y and out 16-byte aligned. */
 int nvfp4_moe_combine(const void* y, const int* row_of_pair, const float* weights, float* out,
                       int tokens, int choices, int hidden, void* stream);
+
+/* Rows of experts that follow one another without padding: offsets[e] (device, `experts` + 1
+ * ints) = pairs of the experts before e, from nvfp4_moe_count's counts, and the placement of every
+ * pair in them (nvfp4_moe_place with the first rows on the device; `rows` at least the pairs).
+ * What nvfp4_int8_group_gemm reads; at most 512 experts. */
+int nvfp4_moe_offsets(const int* counts, int experts, int* offsets, void* stream);
+int nvfp4_moe_place_offsets(const void* ids, int ids_are_64bit, long long pairs, int choices,
+                            int experts, const int* offsets, int rows, int* cursors,
+                            int* row_of_pair, int* token_of_row, void* stream);
+
+/* ---- 8-bit-integer operators ------------------------------------------------------------
+ * Products of INT8 codes with an FP32 scale for each token (row of A) and each output channel
+ * (row of B), beside the block-scaled FP4 ones: no counterpart in the reference, whose 8-bit
+ * products are FP8 (harness/workloads/moe.py:1-33). They keep no plan and no workspace: every
+ * call is one launch on `stream` of the current device, may be captured in a graph, and may be
+ * made from several threads and streams at once.
+ *
+ * D[m][n] = out((float(sum_k A[m][k] B[n][k]) * a_scales[m]) * b_scales[n] + bias[n]), the sum in
+ * 32-bit integers (exact: k is at most 131071), the rest in FP32, rounded once. With `gated`, B
+ * holds n gate rows and then n up rows (b_scales and bias as many) and D = silu(gate) * up.
+ * A and B start and lie (lda, ldb, in bytes) 16-byte aligned; k, n and ldd (elements) are any.
+ * out_kind NVFP4_OUT_F16, _BF16 or _F32. m = 0 launches nothing. */
+int nvfp4_int8_gemm(const void* a, long long lda, const void* b, long long ldb,
+                    const float* a_scales, const float* b_scales, const float* bias, void* d,
+                    long long ldd, int m, int n, int k, int out_kind, int gated, void* stream);
+
+/* The same with rows offsets[e] .. offsets[e + 1] of A, a_scales and D (device, `experts` + 1 ints
+ * that do not decrease) multiplied by expert e's weights, `expert_stride` bytes after the previous
+ * expert's; b_scales [experts][n or 2 n]. Rows of D that no expert owns are left as they were.
+ * Offsets are cut to [0, rows]: no value of theirs reaches outside the buffers. */
+int nvfp4_int8_group_gemm(const void* a, long long lda, const void* b, long long ldb,
+                          long long expert_stride, const float* a_scales, const float* b_scales,
+                          const int* offsets, void* d, long long ldd, int experts, int rows, int n,
+                          int k, int out_kind, int gated, void* stream);
+
+/* Rows of x (FP32, BF16 or FP16, ldx elements apart) -> INT8 codes q (ldq bytes apart) and a scale
+ * for each: scale = max |x| / 127 and code = x / scale to the nearest integer, ties to even, both
+ * quotients correctly rounded. A zero row has scale 0; a row with an infinity or a NaN has that as
+ * its scale and zero codes, so that its products are NaN. With source_rows (device, `rows` ints)
+ * row r is row source_rows[r] of the `tokens` rows of x; where that is negative or beyond them the
+ * row's codes and scale are left as they were. Without, rows = tokens. */
+int nvfp4_int8_quantize(const void* x, int x_kind, long long ldx, const int* source_rows, int rows,
+                        int tokens, int k, void* q, long long ldq, float* scales, void* stream);
+
+/* The end of one block and the start of the next, a row of `hidden` (at most 32768) at a time:
+ *   p = post_weight ? x / rms(x) * post_weight : x        (the norm after the block)
+ *   r = residual_scale * residual + (gate ? gate * p : p) (r in the residual's type)
+ *   y = r / rms(r) * next_weight                          (the norm before the next; of the FP32 r)
+ * with rms(v) = sqrt(mean(v^2) + eps). Weights and gate are FP32; gate [gates][hidden], each row for
+ * tokens / gates consecutive tokens. next_weight may be null (no y); residual may be null, then only
+ * y = x / rms(x) * next_weight is made. y_kind: NVFP4_IN_* or NVFP4_NORM_CODES, INT8 codes and
+ * `scales` as nvfp4_int8_quantize makes them of the FP32 y. r may be the residual itself. */
+#define NVFP4_NORM_CODES (-1)
+int nvfp4_residual_norm(const void* x, int x_kind, long long ldx, const void* residual,
+                        int residual_kind, long long ldres, const float* post_weight,
+                        const float* gate, int gates, float residual_scale,
+                        const float* next_weight, double eps, void* r, long long ldr, void* y,
+                        int y_kind, long long ldy, float* scales, int tokens, int hidden,
+                        void* stream);
 
 /* out[i] = half(silu(h1[i]) * h2[i]) over `size` FP32 elements. Replaces the
  * silu_product kernel (impls/nvfp4_dual_gemm/kernels/silu_product.cu:7-9,

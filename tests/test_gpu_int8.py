@@ -1,0 +1,510 @@
+"""The 8-bit-integer operators on a B200 against plain computations in 64 bits.
+
+Tolerances. ``e`` is the output type's unit (half a step: ``finfo.eps / 2``), ``u = 2**-24`` FP32's.
+A product is ``float(sum) * sa * sb + bias``: the sum is exact, so four FP32 roundings of at most
+the size of the result or of the product before the bias, then one of the output type, and half the
+smallest subnormal step of FP16 where results are that small. The gate multiplies ``silu(g)`` and
+the up product. ``silu`` is ``g * 1/(1 + exp(-g))``: the exponential is documented to ``2 +
+1.173 |g|`` steps of ``2**-23`` and the quotient to 2, and its slope is below 1.1."""
+
+import numpy as np
+import pytest
+import torch
+
+from harness import int8, native
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda:0"
+U = 2.0 ** -24
+FP16_STEP = 2.0 ** -25
+
+
+def rng_of(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def make_codes(g, *shape, extra=0):
+    """Codes of the whole range, -128 included; rows ``extra`` bytes further apart than needed."""
+    *lead, k = shape
+    pitch = -(-k // 16) * 16 + extra
+    return torch.randint(-128, 128, (*lead, pitch), dtype=torch.int8, device=DEV, generator=g)[..., :k]
+
+
+def product_bounds(a, b, sa, sb, bias, gated, dtype):
+    """(value, bound on the error) in 64 bits."""
+    z = (a.double() @ b.double().T) * sa.double()[:, None] * sb.double()
+    err = 4 * U * z.abs()
+    if bias is not None:
+        z = z + bias.double()
+        err = err + 2 * U * (z.abs() + bias.double().abs())
+    if gated:
+        gate, up = z.chunk(2, dim=1)
+        eg, eu = err.chunk(2, dim=1)
+        s = gate * torch.sigmoid(gate)
+        es = 1.1 * eg + s.abs() * ((2 + 1.173 * gate.abs() + 2 + 2) * 2 * U)
+        z = s * up
+        err = es * up.abs() + s.abs() * eu + es * eu + 2 * U * z.abs()
+    e = torch.finfo(dtype).eps / 2
+    return z, err * (1 + e) + e * z.abs() + (FP16_STEP if dtype == torch.float16 else 1e-44)
+
+
+def assert_product(got, a, b, sa, sb, bias=None, gated=False):
+    z, bound = product_bounds(a, b, sa, sb, bias, gated, got.dtype)
+    over = (got.double() - z).abs() - bound
+    assert got.shape == z.shape and not torch.isnan(got).any()
+    assert (over <= 0).all(), f"{over.max().item()} over the bound, at {torch.nonzero(over > 0)[:4].tolist()}"
+
+
+def guarded(rows, n, dtype, pitch=None, lead=3):
+    """An output inside a larger buffer of a known filling; (view, check that the rest kept it)."""
+    pitch = pitch or n + 5
+    buffer = torch.full((rows + 2 * lead, pitch), 77.0, dtype=dtype, device=DEV)
+    view = buffer[lead:lead + rows, 2:2 + n] if pitch > n + 1 else buffer[lead:lead + rows, :n]
+
+    def check():
+        rest = buffer.clone()
+        (rest[lead:lead + rows, 2:2 + n] if pitch > n + 1 else rest[lead:lead + rows, :n]).fill_(77.0)
+        assert (rest == 77.0).all(), "written outside the output"
+    return view, check
+
+
+DTYPES = (torch.bfloat16, torch.float16, torch.float32)
+
+
+@pytest.mark.parametrize("m,n,k", [
+    (1, 1, 1), (1, 8, 16), (1, 300, 7), (2, 129, 130), (7, 64, 128), (16, 128, 256), (17, 127, 1000),
+    (31, 257, 144), (33, 1000, 96), (64, 64, 2048), (65, 33, 4097), (100, 515, 513), (127, 130, 127),
+    (129, 256, 129), (255, 200, 384), (256, 256, 128), (257, 511, 640), (300, 1030, 2064),
+    (513, 770, 1100), (1000, 96, 80), (1, 4096, 4096), (5, 2000, 8192), (40, 136, 16384)])
+@pytest.mark.parametrize("gated", [False, True])
+def test_product_over_sizes(m, n, k, gated):
+    """Odd and small sizes, every output type, an output with rows of its own pitch, and no byte
+    outside it."""
+    g = rng_of(m * 1009 + n * 31 + k)
+    width = 2 * n if gated else n
+    a, b = make_codes(g, m, k, extra=16), make_codes(g, width, k)
+    sa = 0.5 + torch.rand(m, device=DEV, generator=g)
+    sb = (0.5 + torch.rand(width, device=DEV, generator=g)) * (2e-4 / k ** 0.5)
+    bias = torch.randn(width, device=DEV, generator=g)
+    for i, dtype in enumerate(DTYPES):
+        with_bias = bias if i != 0 else None
+        out, check = guarded(m, n, dtype, pitch=n + 5 if i else -(-n // 8) * 8)
+        got = int8.gemm(a, b, sa, sb, bias=with_bias, gated=gated, out_dtype=dtype, out=out)
+        assert got is out
+        assert_product(got, a, b, sa, sb, with_bias, gated)
+        check()
+        again = int8.gemm(a, b, sa, sb, bias=with_bias, gated=gated, out_dtype=dtype)
+        assert torch.equal(again, got), "the same call gave other bits"
+
+
+def test_product_extremes():
+    """All codes -128 at a depth near the largest: the 32-bit sum does not wrap, and FP32 output
+    is it times the scales, rounded as written. Zero, infinite and NaN scales go through."""
+    k = 131056
+    a = torch.full((3, k), -128, dtype=torch.int8, device=DEV)
+    b = torch.full((130, k), -128, dtype=torch.int8, device=DEV)
+    b[1] = 127
+    sa = torch.tensor([1.0, 0.0, 0.5], device=DEV)
+    sb = torch.ones(130, device=DEV)
+    sb[5], sb[6] = float("inf"), float("nan")
+    y = int8.gemm(a, b, sa, sb, out_dtype=torch.float32)
+    assert y[0, 0].item() == k * 128 * 128 and y[2, 0].item() == k * 64 * 128
+    assert y[0, 1].item() == float(np.float32(-k * 128 * 127))
+    assert (y[1, :5] == 0).all() and y[0, 5].item() == float("inf")
+    assert torch.isnan(y[1, 5]) and torch.isnan(y[:, 6]).all()
+    h = int8.gemm(a, b, sa, sb, out_dtype=torch.float16)
+    assert h[0, 0].item() == float("inf")     # beyond FP16: infinite, not the largest value
+
+
+def test_product_of_no_rows_and_of_views():
+    g = rng_of(5)
+    b, sb = make_codes(g, 40, 64), torch.rand(40, device=DEV, generator=g)
+    assert int8.gemm(make_codes(g, 0, 64), b, torch.empty(0, device=DEV), sb).shape == (0, 40)
+    big = make_codes(g, 60, 256)
+    a = big[::3, 32:96]                       # rows 768 bytes apart, from the 32nd byte on
+    wide = make_codes(g, 80, 128)
+    sa = torch.rand(20, device=DEV, generator=g)
+    got = int8.gemm(a, wide[::2, 64:], sa, sb, out_dtype=torch.float32)
+    assert_product(got, a, wide[::2, 64:], sa, sb)
+    with pytest.raises(ValueError):
+        int8.gemm(big[:, 8:72], b, torch.rand(60, device=DEV), sb)     # 8 bytes off
+    with pytest.raises(ValueError):
+        int8.gemm(big[:1].expand(20, 256), make_codes(g, 40, 256), sa, sb)   # rows on top of each other
+    with pytest.raises(ValueError):
+        int8.gemm(a, b.cpu(), sa, sb)
+
+
+@pytest.mark.parametrize("counts,n,k,gated", [
+    ((1,), 8, 16, False), ((0, 0, 3), 100, 64, False), ((0, 0), 16, 32, False),
+    ((5, 0, 130, 1, 0, 64), 72, 100, True), ((257, 3, 129), 136, 528, True), ((64,) * 8, 256, 256, False),
+    ((1, 2, 3, 4, 5, 6, 7, 8, 9), 33, 1000, False), ((700, 0, 1), 513, 300, True),
+    (tuple((i * 7) % 5 for i in range(300)), 24, 48, False), ((16,) * 32, 512, 2048, True)])
+def test_grouped_product(counts, n, k, gated):
+    """Ragged groups, empty ones among them, against each group's product; rows in front of the
+    first group and behind the last keep what the output held."""
+    g = rng_of(sum(counts) + n)
+    experts, owned, front, behind = len(counts), sum(counts), 3, 4
+    width = 2 * n if gated else n
+    rows = front + owned + behind
+    a, b = make_codes(g, rows, k), make_codes(g, experts, width, k)
+    sa = 0.5 + torch.rand(rows, device=DEV, generator=g)
+    sb = (0.5 + torch.rand((experts, width), device=DEV, generator=g)) * (2e-4 / k ** 0.5)
+    edges = [front]
+    for count in counts:
+        edges.append(edges[-1] + count)
+    offsets = torch.tensor(edges, dtype=torch.int32, device=DEV)
+    for dtype in DTYPES:
+        out, check = guarded(rows, n, dtype)
+        int8.grouped_gemm(a, b, sa, sb, offsets, gated=gated, out_dtype=dtype, out=out)
+        check()
+        assert (out[:front] == 77.0).all() and (out[rows - behind:] == 77.0).all()
+        for e, (lo, hi) in enumerate(zip(edges, edges[1:])):
+            if hi > lo:
+                assert_product(out[lo:hi], a[lo:hi], b[e], sa[lo:hi], sb[e], None, gated)
+
+
+def test_grouped_product_of_strided_experts_equals_the_dense_one():
+    g = rng_of(9)
+    b = make_codes(g, 6, 200, 96)[::2]
+    a, counts = make_codes(g, 333, 96), (100, 33, 200)
+    sa = torch.rand(333, device=DEV, generator=g)
+    sb = torch.rand((3, 200), device=DEV, generator=g)
+    offsets = torch.tensor([0, 100, 133, 333], dtype=torch.int32, device=DEV)
+    got = int8.grouped_gemm(a, b, sa, sb, offsets, out_dtype=torch.float32)
+    want = torch.cat([int8.gemm(x, b[e], s, sb[e], out_dtype=torch.float32)
+                      for e, (x, s) in enumerate(zip(a.split(counts), sa.split(counts)))])
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("edges", [(-5, 4, 900), (0, 1 << 30, 1 << 30), (0, 60, 20), (100, 100, 100),
+                                   (-(1 << 31), (1 << 31) - 1, 0)])
+def test_offsets_never_reach_outside_the_rows(edges):
+    """Offsets that no plan would make: cut to the rows of the buffers, and nothing else is
+    written. The rows of the experts that are in order are right."""
+    g = rng_of(3)
+    rows, n, k = 90, 40, 64
+    a, b = make_codes(g, rows, k), make_codes(g, 2, n, k)
+    sa, sb = torch.rand(rows, device=DEV, generator=g), torch.rand((2, n), device=DEV, generator=g)
+    out, check = guarded(rows, n, torch.float32)
+    int8.grouped_gemm(a, b, sa, sb, torch.tensor(edges, dtype=torch.int32, device=DEV),
+                      out_dtype=torch.float32, out=out)
+    torch.cuda.synchronize()
+    check()
+    lo, hi = (min(max(v, 0), rows) for v in edges[:2])
+    if hi > lo:
+        assert_product(out[lo:hi], a[lo:hi], b[0], sa[lo:hi], sb[0])
+
+
+def np_quantized(x):
+    """(codes, scales) with numpy's correctly rounded FP32 divisions."""
+    x = x.float().cpu().numpy()
+    with np.errstate(invalid="ignore", over="ignore", divide="ignore"):
+        scales = (np.abs(x).max(1) / np.float32(127)).astype(np.float32)
+        live = np.isfinite(scales) & (scales > 0)
+        q = np.clip(np.rint(x / np.where(live, scales, 1)[:, None].astype(np.float32)), -127, 127)
+    return np.where(live[:, None], q, 0).astype(np.int8), scales
+
+
+def assert_quantized(got, x):
+    q, s = np_quantized(x)
+    np.testing.assert_array_equal(got[1].cpu().numpy(), s)
+    np.testing.assert_array_equal(got[0].cpu().numpy(), q)
+
+
+@pytest.mark.parametrize("tokens,k", [(1, 1), (1, 2), (3, 7), (2, 8), (5, 63), (4, 64), (33, 255), (9, 1000),
+                                      (300, 1024), (17, 2049), (6, 4096), (5, 5120), (3, 8191), (2, 8192),
+                                      (3, 16384), (2, 16392), (1, 40001), (2, 131071), (1025, 40)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_quantiser_bit_for_bit(tokens, k, dtype):
+    g = rng_of(tokens + k)
+    x = torch.randn((tokens, k), device=DEV, generator=g)
+    x *= torch.exp(2 * torch.randn((tokens, 1), device=DEV, generator=g))
+    x = x.to(dtype)
+    got = int8.quantize_tokens(x)
+    assert got[0].stride(0) % 16 == 0 or tokens == 1
+    assert_quantized(got, x)
+    # Rows that start and lie where no wide load can.
+    padded = torch.zeros((tokens, k + 3), dtype=dtype, device=DEV)
+    padded[:, 1:k + 1] = x
+    assert_quantized(int8.quantize_tokens(padded[:, 1:k + 1]), x)
+    buffer = torch.full((tokens + 2, -(-k // 16) * 16 + 16), 99, dtype=torch.int8, device=DEV)
+    scales = torch.empty(tokens, device=DEV)
+    int8.quantize_tokens(x, out=(buffer[1:tokens + 1, :k], scales))
+    assert_quantized((buffer[1:tokens + 1, :k], scales), x)
+    assert (buffer[:, k:] == 99).all() and (buffer[0] == 99).all() and (buffer[-1] == 99).all()
+
+
+@pytest.mark.parametrize("k", [5, 64, 3000])
+def test_quantiser_of_special_rows(k):
+    """Zero rows, infinities, NaN, subnormals, ties and the largest values."""
+    x = torch.zeros((12, k), device=DEV)
+    x[1, k // 2] = float("inf")
+    x[2, k - 1] = float("-inf")
+    x[3, 0] = float("nan")
+    x[4] = 1e-45
+    x[5] = 1e-40
+    x[5, 1] = -3e-39
+    x[6] = 3.4028234663852886e38
+    x[7] = torch.arange(k, device=DEV) % 255 - 127.0            # exact codes
+    x[8] = (torch.arange(k, device=DEV) % 253 - 126.0) + 0.5    # ties
+    x[8, 0] = 127.0
+    x[9] = -0.0
+    x[10, 0] = -1.0
+    x[11] = 1.0
+    x[11, 2] = float("nan")
+    x[11, 3] = float("inf")
+    q, s = int8.quantize_tokens(x)
+    assert_quantized((q[:11], s[:11]), x[:11])
+    assert torch.isnan(s[11]) and not q[11].any()
+    for bad in (1, 2, 3, 11):        # products of such rows are NaN
+        y = int8.gemm(q[bad:bad + 1], q[7:8], s[bad:bad + 1], s[7:8], out_dtype=torch.float32)
+        assert torch.isnan(y).all()
+
+
+@pytest.mark.parametrize("k", [16, 100, 2880])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_quantiser_gathers(k, dtype):
+    """The same row several times, rows left out, and indices outside: their rows keep what the
+    buffers held."""
+    g = rng_of(k)
+    x = torch.randn((7, k), device=DEV, generator=g).to(dtype)
+    rows = torch.tensor([6, 0, 0, -1, 3, 7, 6, 1 << 30, -(1 << 31), 5], dtype=torch.int32, device=DEV)
+    q = torch.full((10, -(-k // 16) * 16), 55, dtype=torch.int8, device=DEV)[:, :k]
+    s = torch.full((10,), -3.0, device=DEV)
+    int8.quantize_tokens(x, rows=rows, out=(q, s))
+    valid = (rows >= 0) & (rows < 7)
+    assert_quantized((q[valid], s[valid]), x[rows[valid].long()])
+    assert (q[~valid] == 55).all() and (s[~valid] == -3.0).all()
+    assert int8.quantize_tokens(x[:0], rows=rows[3:4], out=(q[3:4], s[3:4]))[1][0] == -3.0
+    empty = int8.quantize_tokens(x, rows=rows[:0])
+    assert empty[0].shape == (0, k) and empty[1].shape == (0,)
+
+
+def norm_plain(x, residual, post, gate, scale, weight, eps):
+    """(r, y, bound of r's error in FP32, bound of y's) in 64 bits."""
+    p = x.double()
+    parts = torch.zeros_like(p)
+    if post is not None:
+        p = p / (p.square().mean(1, keepdim=True) + eps).sqrt() * post.double()
+    if gate is not None:
+        p = p * gate.double().repeat_interleave(x.shape[0] // gate.shape[0], dim=0)
+    r = p
+    parts = 5 * U * p.abs()                 # rstd, two products, the gate, and to spare
+    if residual is not None:
+        r = residual.double() * scale + p
+        parts = parts + 2 * U * (residual.double() * scale).abs() + U * r.abs()
+    if weight is None:
+        return r, None, parts, None
+    rstd = 1 / (r.square().mean(1, keepdim=True) + eps).sqrt()
+    y = r * rstd * weight.double()
+    # An error d of r moves the row's root mean square by at most rms(d).
+    moved = (parts.square().mean(1, keepdim=True).sqrt() * rstd).clamp(max=1.0)
+    return r, y, parts, parts * rstd * weight.double().abs() * (1 + moved) + y.abs() * (moved * (1 + moved) + 4 * U)
+
+
+def assert_norm(outputs, residual_dtype, y_dtype, plain):
+    r, y, scales = outputs
+    want_r, want_y, er, ey = plain
+    if r is not None:
+        e = torch.finfo(residual_dtype).eps / 2
+        assert r.dtype == residual_dtype
+        step = FP16_STEP if residual_dtype == torch.float16 else 1e-40
+        assert ((r.double() - want_r).abs() <= er * (1 + e) + e * want_r.abs() + step).all()
+    if want_y is None:
+        assert y is None and scales is None
+    elif scales is None:
+        e = torch.finfo(y_dtype).eps / 2
+        assert y.dtype == y_dtype
+        step = FP16_STEP if y_dtype == torch.float16 else 1e-40
+        assert ((y.double() - want_y).abs() <= ey * (1 + e) + e * want_y.abs() + step).all()
+    else:
+        assert y.dtype == torch.int8
+        amax, at = want_y.abs().max(1)
+        assert ((scales.double() - amax / 127).abs() <= ey.max(1).values / 127 + U * amax).all()
+        # A code is half a step from its value, and the value off by its own error.
+        off = (y.double() * scales.double()[:, None] - want_y).abs()
+        assert (off <= scales.double()[:, None] * (0.5 + 127 * 4 * U) + ey).all()
+
+
+@pytest.mark.parametrize("tokens,hidden", [(1, 1), (1, 7), (2, 8), (3, 63), (4, 128), (33, 255), (7, 1000),
+                                           (200, 1024), (5, 2049), (6, 2880), (2, 4100), (4, 7168), (3, 8192),
+                                           (2, 10001), (2, 16384), (1, 32767), (2, 32768), (1200, 24)])
+@pytest.mark.parametrize("kind", range(4))
+def test_norm_over_sizes(tokens, hidden, kind):
+    g = rng_of(tokens * 7 + hidden)
+    xt, rt, yt = ((torch.bfloat16, torch.bfloat16, torch.bfloat16), (torch.float32, torch.float16, torch.float32),
+                  (torch.float16, torch.float32, torch.float16), (torch.float32, torch.bfloat16, torch.bfloat16))[kind]
+    x = (3 * torch.randn((tokens, hidden), device=DEV, generator=g)).to(xt)
+    residual = torch.randn((tokens, hidden), device=DEV, generator=g).to(rt)
+    post = 0.5 + torch.rand(hidden, device=DEV, generator=g)
+    weight = 0.5 + torch.rand(hidden, device=DEV, generator=g)
+    gates = {0: 1, 1: tokens, 2: None, 3: 2 if tokens % 2 == 0 else 1}[kind]
+    gate = torch.randn((gates, hidden), device=DEV, generator=g) if gates else None
+    scale = (1.0, 0.5, 0.3, -2.0)[kind]
+    if kind == 2:
+        post = None
+    f32scale = float(np.float32(scale))
+    plain = norm_plain(x, residual, post, gate, f32scale, weight, 1e-6)
+    call = dict(post_weight=post, gate=gate, residual_scale=scale, eps=1e-6)
+    assert_norm(int8.residual_norm(x, residual, next_weight=weight, out_dtype=yt, **call), rt, yt, plain)
+    coded = int8.residual_norm(x, residual, next_weight=weight, quantize=True, **call)
+    assert_norm(coded, rt, None, plain)
+    assert_norm(int8.residual_norm(x, residual, **call), rt, None, (*plain[:1], None, plain[2], None))
+    # The codes are those of the FP32 rows.
+    y32 = int8.residual_norm(x, residual, next_weight=weight, out_dtype=torch.float32, **call)[1]
+    assert_quantized(coded[1:], y32)
+    # The norm alone.
+    alone = norm_plain(x, None, None, None, 1.0, weight, 1e-6)
+    assert_norm(int8.residual_norm(x, next_weight=weight, out_dtype=yt), None, yt, alone)
+    # In place, from rows that start and lie where no wide load can.
+    off = torch.zeros((tokens, hidden + 3), dtype=rt, device=DEV)
+    off[:, 1:hidden + 1] = residual
+    xoff = torch.zeros((tokens, hidden + 5), dtype=xt, device=DEV)
+    xoff[:, 3:hidden + 3] = x
+    inplace = int8.residual_norm(xoff[:, 3:hidden + 3], off[:, 1:hidden + 1], next_weight=weight, quantize=True,
+                                 residual_out=off[:, 1:hidden + 1], **call)
+    assert torch.equal(inplace[0], coded[0]) and torch.equal(inplace[1], coded[1])
+    assert torch.equal(inplace[2], coded[2])
+    assert (off[:, 0] == 0).all() and (off[:, hidden + 1:] == 0).all()
+
+
+def test_norm_of_special_rows():
+    """Zero rows give zeros, infinite and NaN rows poison only themselves."""
+    x = torch.ones((5, 300), device=DEV)
+    x[0] = 0
+    x[1, 7] = float("inf")
+    x[2, 299] = float("nan")
+    x[3] = 1e30                          # the square overflows FP32, not the sum in 64 bits
+    w = torch.full((300,), 2.0, device=DEV)
+    _, y, _ = int8.residual_norm(x, next_weight=w, eps=1e-6)
+    assert (y[0] == 0).all() and torch.isnan(y[1, 7]) and (y[1, :7] == 0).all() and torch.isnan(y[2]).all()
+    torch.testing.assert_close(y[3], torch.full((300,), 2.0, device=DEV), rtol=4 * U, atol=0)
+    _, q, s = int8.residual_norm(x, next_weight=w, quantize=True)
+    assert s[0] == 0 and not q[:3].any() and torch.isnan(s[1]) and torch.isnan(s[2])
+    assert (q[3:] == 127).all()
+    assert int8.residual_norm(x[:0], next_weight=w)[1].shape == (0, 300)
+    with pytest.raises(ValueError):
+        int8.residual_norm(x, x, gate=torch.ones((2, 300), device=DEV), next_weight=w)
+
+
+def test_calls_on_two_streams_and_from_two_threads():
+    """Nothing is shared between calls: two streams at once give what one gives."""
+    import threading
+
+    g = rng_of(21)
+    sets = []
+    for m, n, k in ((200, 1000, 4096), (3, 4000, 2048)):
+        x = torch.randn((m, k), device=DEV, generator=g)
+        b, sb = int8.quantize_tokens(torch.randn((n, k), device=DEV, generator=g))
+        a, sa = int8.quantize_tokens(x)
+        sets.append((x, b, sb, int8.gemm(a, b, sa, sb)))
+    torch.cuda.synchronize()
+    results, errors = [[], []], []
+
+    def work(i):
+        try:
+            stream = torch.cuda.Stream(DEV)
+            x, b, sb, _ = sets[i]
+            with torch.cuda.stream(stream):
+                for _ in range(20):
+                    a, sa = int8.quantize_tokens(x)
+                    results[i].append(int8.gemm(a, b, sa, sb))
+            stream.synchronize()
+        except Exception as error:
+            errors.append(error)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+    for (*_, want), got in zip(sets, results):
+        assert len(got) == 20 and all(torch.equal(y, want) for y in got)
+
+
+def test_a_captured_chain_replays_on_new_data():
+    """Norm, product, quantiser and grouped product in one graph, replayed with other inputs and
+    other offsets, equal the eager calls; two graphs of the same calls share nothing."""
+    g = rng_of(31)
+    tokens, hidden, inter, experts = 50, 192, 80, 4
+    w = torch.rand(hidden, device=DEV, generator=g)
+    b1, s1 = int8.quantize_tokens(torch.randn((2 * inter, hidden), device=DEV, generator=g))
+    b2, s2 = int8.quantize_tokens(torch.randn((experts * hidden, inter), device=DEV, generator=g))
+    b2 = torch.nn.functional.pad(b2, (0, 0)).contiguous().view(experts, hidden, inter)
+    s2 = s2.view(experts, hidden)
+
+    def chain(x, residual, offsets):
+        r, q, s = int8.residual_norm(x, residual, post_weight=w, next_weight=w, quantize=True)
+        h = int8.gemm(q, b1, s, s1, gated=True)
+        q2, t = int8.quantize_tokens(h)
+        return r, int8.grouped_gemm(q2, b2, t, s2, offsets, out_dtype=torch.float32)
+
+    def inputs(seed):
+        g = rng_of(seed)
+        edges = [0, *sorted(torch.randint(0, tokens + 1, (experts - 1,), generator=torch.Generator().manual_seed(seed)).tolist()), tokens]
+        return (torch.randn((tokens, hidden), device=DEV, generator=g),
+                torch.randn((tokens, hidden), device=DEV, generator=g).bfloat16(),
+                torch.tensor(edges, dtype=torch.int32, device=DEV))
+
+    graphs = []
+    for seed in (1, 2):
+        static = inputs(seed)
+        side = torch.cuda.Stream()
+        with torch.cuda.stream(side):
+            chain(*static)
+        side.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outputs = chain(*static)
+        graphs.append((graph, static, outputs))
+    for seed in (3, 4):
+        fresh = [inputs(seed + 10 * i) for i in range(2)]
+        for (graph, static, _), new in zip(graphs, fresh):
+            for old, value in zip(static, new):
+                old.copy_(value)
+        streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+        torch.cuda.synchronize()
+        for (graph, *_), stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for (_, _, outputs), new in zip(graphs, fresh):
+            for got, want in zip(outputs, chain(*new)):
+                assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("name", ["int8_gemm", "int8_group_gemm", "int8_quantize", "residual_norm"])
+def test_workload_smoke_cases(name):
+    from harness import get_workload
+
+    with get_workload(name).from_arch("sm_100a", device="cuda") as workload:
+        for case in workload.get_cases():
+            if case.suite != "smoke":
+                continue
+            inputs = workload.get_inputs(case)
+            out = workload.run(inputs)
+            workload.validate(workload.get_reference(inputs), out)
+            launch, _ = workload.prepare(inputs)
+            workload.validate(out, launch())
+
+
+def test_offsets_and_placement_of_pairs():
+    """Unpadded routing on the device: offsets are the prefix of the counts, every pair has a row
+    of its expert, ids outside have none."""
+    ids = torch.tensor([[3, 0], [3, 9], [-1, 0], [3, 1]], dtype=torch.int64, device=DEV)
+    stream = torch.cuda.current_stream().cuda_stream
+    counts, cursors = (torch.zeros(5, dtype=torch.int32, device=DEV) for _ in range(2))
+    offsets = torch.full((6,), -7, dtype=torch.int32, device=DEV)
+    row_of_pair, token_of_row = (torch.full((8,), -9, dtype=torch.int32, device=DEV) for _ in range(2))
+    native.moe_count(ids.data_ptr(), True, 8, 5, counts.data_ptr(), stream)
+    native.moe_offsets(counts.data_ptr(), 5, offsets.data_ptr(), stream)
+    native.moe_place_offsets(ids.data_ptr(), True, 8, 2, 5, offsets.data_ptr(), 8, cursors.data_ptr(),
+                             row_of_pair.data_ptr(), token_of_row.data_ptr(), stream)
+    assert offsets.tolist() == [0, 2, 3, 3, 6, 6]
+    rows = row_of_pair.tolist()
+    assert sorted(rows[i] for i in (0, 2, 6)) == [3, 4, 5] and sorted(rows[i] for i in (1, 5)) == [0, 1]
+    assert rows[7] == 2 and rows[3] == rows[4] == -1
+    tokens = token_of_row.tolist()
+    assert all(tokens[rows[i]] == i // 2 for i in (0, 1, 2, 5, 6, 7)) and tokens[6:] == [-1, -1]

@@ -1,0 +1,173 @@
+"""The 8-bit-integer operators without a GPU: what the functions of ``harness.int8`` and the C
+entry points refuse, before anything is launched, and the torch references of their workloads
+against the definitions in 64 bits."""
+
+import numpy as np
+import pytest
+import torch
+
+from harness import get_workload, int8, native
+from harness.workloads import int8 as references
+
+
+@pytest.fixture(scope="module")
+def library():
+    if not native.LIBRARY_PATH.is_file():
+        from harness import build
+        build.build()
+    return native.load()
+
+
+def codes(*shape):
+    return torch.zeros(shape, dtype=torch.int8)
+
+
+def ones(*shape):
+    return torch.ones(shape)
+
+
+def test_functions_refuse_what_they_cannot_take():
+    """Every refusal is a ValueError of the host; what passes the checks ends at the device, which
+    is none here."""
+    a, b, sa, sb = codes(3, 32), codes(8, 32), ones(3), ones(8)
+    for call in (
+        lambda: int8.gemm(a, codes(8, 48), sa, sb),                       # depths differ
+        lambda: int8.gemm(a.float(), b, sa, sb),                          # not codes
+        lambda: int8.gemm(a, b, ones(4), sb),                             # a scale too many
+        lambda: int8.gemm(a, b, sa.half(), sb),
+        lambda: int8.gemm(a, b, sa, ones(16)[::2]),
+        lambda: int8.gemm(a, codes(7, 32), sa, ones(7), gated=True),      # an odd pair
+        lambda: int8.gemm(a, b, sa, sb, bias=ones(4)),
+        lambda: int8.gemm(a, b, sa, sb, out_dtype=torch.float64),
+        lambda: int8.gemm(codes(32, 3).T, b, sa, sb),                     # columns, not rows
+        lambda: int8.gemm(a, b, sa.clone().requires_grad_(), sb),
+        lambda: int8.grouped_gemm(a, codes(2, 8, 32), sa, ones(2, 8), torch.zeros(3, dtype=torch.int64)),
+        lambda: int8.grouped_gemm(a, codes(2, 8, 32), sa, ones(2, 8), torch.zeros(2, dtype=torch.int32)),
+        lambda: int8.grouped_gemm(a, codes(2, 8, 32), sa, ones(16), torch.zeros(3, dtype=torch.int32)),
+        lambda: int8.quantize_tokens(ones(4)),
+        lambda: int8.quantize_tokens(ones(4, 4).double()),
+        lambda: int8.quantize_tokens(ones(4, 4).T[:, ::2]),
+        lambda: int8.quantize_tokens(ones(4, 4), rows=torch.zeros(4, dtype=torch.int64)),
+        lambda: int8.residual_norm(ones(4, 8)),                           # nothing to make
+        lambda: int8.residual_norm(ones(4, 8), ones(4, 9), next_weight=ones(8)),
+        lambda: int8.residual_norm(ones(4, 8), ones(4, 8), post_weight=ones(9)),
+        lambda: int8.residual_norm(ones(4, 8), ones(4, 8), gate=ones(2, 9), next_weight=ones(8)),
+        lambda: int8.residual_norm(ones(4, 8), ones(4, 8), quantize=True),
+        lambda: int8.residual_norm(ones(4, 8), ones(4, 8), next_weight=ones(8), quantize=True,
+                                   out_dtype=torch.float16),
+        lambda: int8.residual_norm(ones(4, 8), next_weight=ones(8), residual_out=ones(4, 8)),
+    ):
+        with pytest.raises(ValueError):
+            call()
+    for call in (lambda: int8.gemm(a, b, sa, sb),
+                 lambda: int8.quantize_tokens(ones(4, 4)),
+                 lambda: int8.residual_norm(ones(4, 8), next_weight=ones(8))):
+        with pytest.raises(RuntimeError):
+            call()
+
+
+def test_entry_points_refuse_before_cuda(library):
+    """Addresses here are never followed: each call is wrong in one argument."""
+    def gemm(a=16, lda=32, b=32, ldb=32, sa=16, sb=16, bias=None, d=16, ldd=8, m=4, n=8, k=32, out=0):
+        return library.nvfp4_int8_gemm(a, lda, b, ldb, sa, sb, bias, d, ldd, m, n, k, out, 0, None)
+
+    assert gemm(a=None) == native.E_INVALID_ARGUMENT
+    assert gemm(d=None) == native.E_INVALID_ARGUMENT
+    assert gemm(out=7) == native.E_INVALID_ARGUMENT
+    assert gemm(lda=16) == native.E_INVALID_ARGUMENT
+    assert gemm(ldb=0) == native.E_INVALID_ARGUMENT
+    assert gemm(ldd=4) == native.E_INVALID_ARGUMENT
+    assert gemm(m=-1) == native.E_UNSUPPORTED_SHAPE
+    assert gemm(n=0) == native.E_UNSUPPORTED_SHAPE
+    assert gemm(k=0) == native.E_UNSUPPORTED_SHAPE
+    assert gemm(k=131072, lda=131072, ldb=131072) == native.E_UNSUPPORTED_SHAPE
+    assert gemm(a=24) == native.E_MISALIGNED
+    assert gemm(lda=40) == native.E_MISALIGNED
+    assert gemm(sa=18) == native.E_MISALIGNED
+    assert gemm(bias=2) == native.E_MISALIGNED
+    assert gemm(d=18, out=native.OUT_F32) == native.E_MISALIGNED
+    assert gemm(m=0, a=None) == 0
+
+    def grouped(offsets=16, experts=2, stride=256, rows=4):
+        return library.nvfp4_int8_group_gemm(16, 32, 16, 32, stride, 16, 16, offsets, 16, 8, experts,
+                                             rows, 8, 32, 0, 0, None)
+
+    assert grouped(offsets=None) == native.E_INVALID_ARGUMENT
+    assert grouped(experts=0) == native.E_UNSUPPORTED_SHAPE
+    assert grouped(experts=1025) == native.E_UNSUPPORTED_SHAPE
+    assert grouped(stride=-256) == native.E_INVALID_ARGUMENT
+    assert grouped(stride=8) == native.E_MISALIGNED
+    assert grouped(offsets=18) == native.E_MISALIGNED
+    assert grouped(rows=0) == 0
+
+    def quantize(x=16, kind=0, ldx=8, source=None, rows=4, tokens=4, k=8, q=16, ldq=16, scales=16):
+        return library.nvfp4_int8_quantize(x, kind, ldx, source, rows, tokens, k, q, ldq, scales, None)
+
+    assert quantize(x=None) == native.E_INVALID_ARGUMENT
+    assert quantize(kind=3) == native.E_INVALID_ARGUMENT
+    assert quantize(rows=5) == native.E_INVALID_ARGUMENT
+    assert quantize(ldx=0) == native.E_INVALID_ARGUMENT
+    assert quantize(ldq=4) == native.E_INVALID_ARGUMENT
+    assert quantize(k=0) == native.E_UNSUPPORTED_SHAPE
+    assert quantize(x=18) == native.E_MISALIGNED
+    assert quantize(rows=0, tokens=0) == 0
+
+    def norm(x=16, residual=16, r=16, post=None, gate=None, gates=0, scale=1.0, weight=16, eps=1e-6,
+             y=16, y_kind=0, scales=None, tokens=4, hidden=8, ldx=8, ldr=8):
+        return library.nvfp4_residual_norm(x, 0, ldx, residual, 0, 8, post, gate, gates, scale, weight,
+                                           eps, r, ldr, y, y_kind, 8, scales, tokens, hidden, None)
+
+    assert norm(x=None) == native.E_INVALID_ARGUMENT
+    assert norm(r=None) == native.E_INVALID_ARGUMENT
+    assert norm(y=None) == native.E_INVALID_ARGUMENT
+    assert norm(y_kind=native.NORM_CODES) == native.E_INVALID_ARGUMENT
+    assert norm(y_kind=5) == native.E_INVALID_ARGUMENT
+    assert norm(eps=0.0) == native.E_INVALID_ARGUMENT
+    assert norm(eps=float("nan")) == native.E_INVALID_ARGUMENT
+    assert norm(residual=None, r=None, post=16) == native.E_INVALID_ARGUMENT
+    assert norm(residual=None, r=None, scale=0.5) == native.E_INVALID_ARGUMENT
+    assert norm(ldx=4) == native.E_INVALID_ARGUMENT
+    assert norm(ldr=0) == native.E_INVALID_ARGUMENT
+    assert norm(gate=16, gates=3) == native.E_UNSUPPORTED_SHAPE
+    assert norm(hidden=32769) == native.E_UNSUPPORTED_SHAPE
+    assert norm(x=18) == native.E_MISALIGNED
+    assert norm(tokens=0, x=None) == 0
+
+    assert library.nvfp4_moe_offsets(None, 4, 16, None) == native.E_INVALID_ARGUMENT
+    assert library.nvfp4_moe_offsets(16, 0, 16, None) == native.E_UNSUPPORTED_SHAPE
+    assert library.nvfp4_moe_place_offsets(16, 1, 8, 2, 4, None, 8, 16, 16, 16, None) == \
+        native.E_INVALID_ARGUMENT
+    assert library.nvfp4_moe_place_offsets(16, 1, 8, 2, 4, 16, 7, 16, 16, 16, None) == \
+        native.E_INVALID_ARGUMENT      # fewer rows than pairs
+
+
+def test_workloads_are_registered_with_cases():
+    for name in ("int8_gemm", "int8_group_gemm", "int8_quantize", "residual_norm"):
+        workload = get_workload(name)(None, device="cpu")
+        cases = workload.get_cases()
+        assert len({c.name for c in cases}) == len(cases) > 3
+        case = cases[1]
+        inputs = workload.get_inputs(case)
+        reference = workload.get_reference(inputs)
+        workload.validate(reference, workload.get_reference(workload.get_inputs(case)))
+        with pytest.raises(RuntimeError):
+            workload.run(inputs)
+
+
+def test_quantiser_reference_is_the_definition():
+    """Scale and codes by numpy's correctly rounded FP32 division."""
+    rng = np.random.default_rng(0)
+    x = (rng.standard_normal((9, 50)) * rng.lognormal(0, 3, (9, 1))).astype(np.float32)
+    x[2] = 0
+    x[4, 7] = np.inf
+    x[5, 3] = np.nan
+    x[6] = 1e-45
+    q, s = references.quantized(torch.from_numpy(x))
+    for row, codes_, scale in zip(x, q.numpy(), s.numpy()):
+        amax = np.abs(row).max()
+        want = np.float32(amax) / np.float32(127)
+        np.testing.assert_array_equal(scale, want)
+        if want > 0 and np.isfinite(want):
+            np.testing.assert_array_equal(codes_, np.clip(np.rint(row / want), -127, 127))
+        else:
+            assert not codes_.any()
