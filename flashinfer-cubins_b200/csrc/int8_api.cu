@@ -9,6 +9,7 @@
 
 #include <cuda_runtime.h>
 
+#include "int8_gemm_kernel.cuh"
 #include "int8_kernels.cuh"
 #include "nvfp4_host.h"
 
@@ -41,15 +42,28 @@ bool is_in_kind(int kind) {
 
 // Sums of k products of two codes of -128..127 stay below 2^31 up to here.
 constexpr int kMaxDepth = 131071;
-constexpr int kMaxExperts = 1024;
 constexpr int kMaxHidden = 32768;
 
-int check_product(const Int8GemmParams& p, int width) {
-  if (p.rows < 0 || p.n < 1 || p.k < 1 || p.k > kMaxDepth || p.experts < 1 ||
-      p.experts > kMaxExperts || width > (1 << 30)) {
+// One product, dense (offsets null, one expert) or grouped.
+struct Product {
+  const void* a;
+  const void* b;
+  const float* a_scales;
+  const float* b_scales;
+  const float* bias;
+  const int* offsets;
+  void* d;
+  long long lda, ldb, expert_stride, ldd;
+  int rows, n, k, experts, out_kind;
+  bool gated;
+};
+
+int check_product(const Product& p) {
+  if (p.rows < 0 || p.n < 1 || p.n > (1 << 30) || p.k < 1 || p.k > kMaxDepth || p.experts < 1 ||
+      p.experts > kInt8MaxExperts) {
     return fail(NVFP4_E_UNSUPPORTED_SHAPE,
                 "unsupported product: %d rows, n=%d, k=%d (at most %d), %d experts (at most %d)",
-                p.rows, p.n, p.k, kMaxDepth, p.experts, kMaxExperts);
+                p.rows, p.n, p.k, kMaxDepth, p.experts, kInt8MaxExperts);
   }
   if (p.rows == 0) return 0;
   if (p.a == nullptr || p.b == nullptr || p.a_scales == nullptr || p.b_scales == nullptr ||
@@ -59,34 +73,120 @@ int check_product(const Int8GemmParams& p, int width) {
   if (p.out_kind != NVFP4_OUT_F16 && p.out_kind != NVFP4_OUT_F32 && p.out_kind != NVFP4_OUT_BF16) {
     return fail(NVFP4_E_INVALID_ARGUMENT, "unknown output kind %d", p.out_kind);
   }
-  if (p.lda < p.k || p.ldb < p.k || p.ldd < p.n || p.expert_stride < 0) {
-    return fail(NVFP4_E_INVALID_ARGUMENT, "rows overlap: lda=%lld ldb=%lld ldd=%lld", p.lda, p.ldb,
-                p.ldd);
+  const long long width = p.gated ? 2ll * p.n : p.n;
+  if (p.lda < p.k || p.ldb < p.k || p.ldd < p.n ||
+      (p.experts > 1 && p.expert_stride < (width - 1) * p.ldb + p.k)) {
+    return fail(NVFP4_E_INVALID_ARGUMENT, "rows overlap: lda=%lld ldb=%lld ldd=%lld, experts %lld apart",
+                p.lda, p.ldb, p.ldd, p.expert_stride);
   }
   if (!aligned(p.a, 16) || !aligned(p.b, 16) || p.lda % 16 != 0 || p.ldb % 16 != 0 ||
-      p.expert_stride % 16 != 0 || !aligned(p.a_scales, 4) || !aligned(p.b_scales, 4) ||
-      !aligned(p.bias, 4) || !aligned(p.offsets, 4) ||
+      (p.experts > 1 && p.expert_stride % 16 != 0) || !aligned(p.a_scales, 4) ||
+      !aligned(p.b_scales, 4) || !aligned(p.bias, 4) || !aligned(p.offsets, 4) ||
       !aligned(p.d, p.out_kind == NVFP4_OUT_F32 ? 4 : 2)) {
     return fail(NVFP4_E_MISALIGNED, "codes must start and lie 16-byte aligned");
   }
   return 0;
 }
 
-int launch_product(const Int8GemmParams& p, int gated, void* stream) {
-  const int width = gated ? 2 * p.n : p.n;
-  if (p.n > (1 << 29)) return fail(NVFP4_E_UNSUPPORTED_SHAPE, "n=%d is too large", p.n);
-  if (int rc = check_product(p, width)) return rc;
-  if (p.rows == 0) return 0;
-  const int tiles = (p.rows + kTile - 1) / kTile + p.experts - 1;
-  const dim3 grid((p.n + kTile - 1) / kTile, tiles);
-  if (tiles > 65535) return fail(NVFP4_E_UNSUPPORTED_SHAPE, "too many rows: %d", p.rows);
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (gated) {
-    int8_gemm_kernel<true><<<grid, 256, 0, s>>>(p);
-  } else {
-    int8_gemm_kernel<false><<<grid, 256, 0, s>>>(p);
+using TileKernel = void (*)(Int8TileParams);
+
+TileKernel tile_kernel(int ctas, bool gated) {
+  if (ctas == 2) return gated ? int8_tile_kernel<2, true> : int8_tile_kernel<2, false>;
+  return gated ? int8_tile_kernel<1, true> : int8_tile_kernel<1, false>;
+}
+
+// Static shared memory of the kernels (the same in all four, to within padding) and the slack that
+// aligns the stages to 1,024 bytes come off what a block can have.
+constexpr int kSharedLimit = 232448;
+constexpr int kStaticShared = 10 * 1024;
+
+int encode(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims,
+           const cuuint64_t* strides, const cuuint32_t* box) {
+  EncodeTiled encoder = nullptr;
+  if (int rc = host_encoder(&encoder)) return rc;
+  const cuuint32_t ones[4] = {1, 1, 1, 1};
+  const CUresult res = encoder(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, rank, const_cast<void*>(base), dims,
+                               strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (res != CUDA_SUCCESS) {
+    return fail(static_cast<int>(res), "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(res));
   }
-  CUDA_TRY(cudaGetLastError());
+  return 0;
+}
+
+int launch_product(const Product& q, void* stream) {
+  if (int rc = check_product(q)) return rc;
+  if (q.rows == 0) return 0;
+  const int sms = host_sm_count();
+  const int k_tiles = (q.k + 127) / 128;
+  const int per_group = (q.rows + q.experts - 1) / q.experts;
+  int ctas = per_group > 128 ? 2 : 1;
+  int tile_tokens = ctas == 2 ? 256 : per_group <= 32 ? 32 : per_group <= 64 ? 64 : 128;
+  int split = 1;
+  const int channels = (q.gated ? 64 : 128) * ctas;
+  const long long n_tiles = (q.n + channels - 1) / channels;
+  // No routing makes more token tiles than this.
+  const long long m_tiles = q.rows / tile_tokens + std::min(q.experts, q.rows);
+  long long tiles = (q.experts == 1 ? (q.rows + tile_tokens - 1) / tile_tokens : m_tiles) * n_tiles;
+  if (ctas == 1) {
+    while (split < 8 && tiles * split * 2 <= sms && split * 2 <= k_tiles) split *= 2;
+  }
+
+  Int8TileParams p{};
+  const cuuint64_t b_dims[4] = {static_cast<cuuint64_t>(q.k), static_cast<cuuint64_t>(q.n),
+                                q.gated ? 2u : 1u, static_cast<cuuint64_t>(q.experts)};
+  const cuuint64_t half = static_cast<cuuint64_t>(q.n) * q.ldb;
+  const cuuint64_t b_strides[3] = {static_cast<cuuint64_t>(q.ldb), half,
+                                   q.experts > 1 ? static_cast<cuuint64_t>(q.expert_stride) : 2 * half};
+  const cuuint32_t b_box[4] = {128, q.gated ? 16u : 128u, q.gated ? 2u : 1u, 1};
+  if (int rc = encode(&p.map_b, q.b, 4, b_dims, b_strides, b_box)) return rc;
+  const cuuint64_t a_dims[2] = {static_cast<cuuint64_t>(q.k), static_cast<cuuint64_t>(q.rows)};
+  const cuuint64_t a_strides[1] = {static_cast<cuuint64_t>(q.lda)};
+  const cuuint32_t a_box[2] = {128, static_cast<cuuint32_t>(tile_tokens / ctas)};
+  if (int rc = encode(&p.map_a, q.a, 2, a_dims, a_strides, a_box)) return rc;
+  const cuuint32_t part_box[2] = {128, static_cast<cuuint32_t>(32 / ctas)};
+  if (int rc = encode(&p.map_a_part, q.a, 2, a_dims, a_strides, part_box)) return rc;
+  p.a_scales = q.a_scales;
+  p.b_scales = q.b_scales;
+  p.bias = q.bias;
+  p.offsets = q.offsets;
+  p.d = q.d;
+  p.ldd = q.ldd;
+  p.rows = q.rows;
+  p.n = q.n;
+  p.k = q.k;
+  p.experts = q.experts;
+  p.out_kind = q.out_kind;
+  p.tile_tokens = tile_tokens;
+  p.split = split;
+  const int stage_bytes = kInt8WeightBytes + tile_tokens / ctas * 128;
+  p.stages = std::min(kInt8MaxStages, (kSharedLimit - kStaticShared - 1024) / stage_bytes);
+  const size_t shared = static_cast<size_t>(p.stages) * stage_bytes + 1024;
+
+  const TileKernel kernel = tile_kernel(ctas, q.gated);
+  CUDA_TRY(cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                kSharedLimit - kStaticShared));
+  const int group = split > 1 ? split : ctas;
+  // A split tile is a cluster's only one; otherwise a CTA (or pair) on every SM walks the tiles.
+  const long long groups = split > 1 ? tiles : std::min<long long>(tiles, sms / ctas);
+  cudaLaunchAttribute attribute[2];
+  attribute[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attribute[0].val.programmaticStreamSerializationAllowed = 1;
+  attribute[1].id = cudaLaunchAttributeClusterDimension;
+  attribute[1].val.clusterDim.x = static_cast<unsigned int>(group);
+  attribute[1].val.clusterDim.y = 1;
+  attribute[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(static_cast<unsigned int>(groups * group));
+  config.blockDim = dim3(kInt8Threads);
+  config.dynamicSmemBytes = shared;
+  config.stream = static_cast<cudaStream_t>(stream);
+  config.attrs = attribute;
+  config.numAttrs = group > 1 ? 2 : 1;
+  void* args[1] = {&p};
+  CUDA_TRY(cudaLaunchKernelExC(&config, reinterpret_cast<const void*>(kernel), args));
   return 0;
 }
 
@@ -104,22 +204,9 @@ extern "C" {
 int nvfp4_int8_gemm(const void* a, long long lda, const void* b, long long ldb,
                     const float* a_scales, const float* b_scales, const float* bias, void* d,
                     long long ldd, int m, int n, int k, int out_kind, int gated, void* stream) {
-  Int8GemmParams p{};
-  p.a = static_cast<const int8_t*>(a);
-  p.b = static_cast<const int8_t*>(b);
-  p.a_scales = a_scales;
-  p.b_scales = b_scales;
-  p.bias = bias;
-  p.d = d;
-  p.lda = lda;
-  p.ldb = ldb;
-  p.ldd = ldd;
-  p.rows = m;
-  p.n = n;
-  p.k = k;
-  p.experts = 1;
-  p.out_kind = out_kind;
-  return launch_product(p, gated, stream);
+  const Product q{a, b, a_scales, b_scales, bias, nullptr, d, lda, ldb, 0, ldd,
+                  m, n, k, 1, out_kind, gated != 0};
+  return launch_product(q, stream);
 }
 
 int nvfp4_int8_group_gemm(const void* a, long long lda, const void* b, long long ldb,
@@ -127,23 +214,25 @@ int nvfp4_int8_group_gemm(const void* a, long long lda, const void* b, long long
                           const int* offsets, void* d, long long ldd, int experts, int rows, int n,
                           int k, int out_kind, int gated, void* stream) {
   if (offsets == nullptr && rows > 0) return fail(NVFP4_E_INVALID_ARGUMENT, "null operand");
-  Int8GemmParams p{};
-  p.a = static_cast<const int8_t*>(a);
-  p.b = static_cast<const int8_t*>(b);
-  p.a_scales = a_scales;
-  p.b_scales = b_scales;
-  p.offsets = offsets;
-  p.d = d;
-  p.lda = lda;
-  p.ldb = ldb;
-  p.expert_stride = expert_stride;
-  p.ldd = ldd;
-  p.rows = rows;
-  p.n = n;
-  p.k = k;
-  p.experts = experts;
-  p.out_kind = out_kind;
-  return launch_product(p, gated, stream);
+  const Product q{a, b, a_scales, b_scales, nullptr, offsets, d, lda, ldb, expert_stride, ldd,
+                  rows, n, k, experts, out_kind, gated != 0};
+  return launch_product(q, stream);
+}
+
+int nvfp4_int8_status(void* stream, int* status) {
+  if (status == nullptr) return fail(NVFP4_E_INVALID_ARGUMENT, "null argument");
+  *status = 0;
+  void* word = nullptr;
+  CUDA_TRY(cudaGetSymbolAddress(&word, g_int8_status));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  int value = 0;
+  CUDA_TRY(cudaMemcpyAsync(&value, word, sizeof(int), cudaMemcpyDeviceToHost, s));
+  CUDA_TRY(cudaStreamSynchronize(s));
+  *status = value;
+  if (value == 0) return 0;
+  CUDA_TRY(cudaMemsetAsync(word, 0, sizeof(int), s));
+  CUDA_TRY(cudaStreamSynchronize(s));
+  return fail(NVFP4_E_DEVICE_TIMEOUT, "an INT8 product abandoned a bounded wait (code %d)", value);
 }
 
 int nvfp4_int8_quantize(const void* x, int x_kind, long long ldx, const int* source_rows, int rows,
@@ -248,10 +337,10 @@ int nvfp4_residual_norm(const void* x, int x_kind, long long ldx, const void* re
 
 int nvfp4_moe_offsets(const int* counts, int experts, int* offsets, void* stream) {
   if (counts == nullptr || offsets == nullptr) return fail(NVFP4_E_INVALID_ARGUMENT, "null operand");
-  if (experts < 1 || experts > kMaxExperts) {
-    return fail(NVFP4_E_UNSUPPORTED_SHAPE, "%d experts (at most %d)", experts, kMaxExperts);
+  if (experts < 1 || experts > kInt8MaxExperts) {
+    return fail(NVFP4_E_UNSUPPORTED_SHAPE, "%d experts (at most %d)", experts, kInt8MaxExperts);
   }
-  expert_offsets_kernel<<<1, kMaxExperts, 0, static_cast<cudaStream_t>(stream)>>>(counts, experts,
+  expert_offsets_kernel<<<1, kInt8MaxExperts, 0, static_cast<cudaStream_t>(stream)>>>(counts, experts,
                                                                                   offsets);
   CUDA_TRY(cudaGetLastError());
   return 0;

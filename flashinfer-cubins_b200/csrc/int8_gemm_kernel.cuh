@@ -1,0 +1,559 @@
+// Products of INT8 codes on the tensor cores, dense or over ragged groups of rows:
+//   D[m][c] = out((float(sum_k A[m][k] B[c][k]) * a_scales[m]) * b_scales[c] + bias[c])
+// and with a gate silu of that for gate channels times that for up channels.
+//
+// The tile lies on its side: channels (rows of B, the weights) are the MMA's 128 rows, tokens
+// (rows of A) its columns. A few tokens then cost a narrow MMA instead of an empty tile, the
+// weights stream through the wide operand, and in the epilogue a warp holds 32 neighbouring
+// channels of one token at a time, which are neighbours in D: every store instruction of a warp
+// is one run of 64 or 128 bytes, for any n, ldd and alignment, with no staging.
+//
+// Warps of a CTA (192 threads): 0 loads (one thread issues cp.async.bulk.tensor into a ring of
+// stages of 128 k), 1 issues tcgen05.mma.kind::i8 (32 k each) into one of two accumulators in
+// tensor memory, 2-5 take the other accumulator out, scale and store it. CTAS = 2: a pair of CTAs
+// on neighbouring SMs works on 256 channel rows with tcgen05.mma.cta_group::2; each loads its own
+// 128 rows of B and half of the tile's tokens.
+//
+// GATED: of a CTA's 128 rows every 32 are 16 gate channels and the same 16 up channels (the tensor
+// map has gate and up as a dimension of its own, so one copy brings both). A warp of the epilogue
+// then holds both of 16 channels, lanes 16 apart, and exchanges two tokens' values in one shuffle.
+//
+// SPLIT (cluster of `split` CTAs, one tile each cluster): each CTA takes a part of k, the partial
+// sums meet in shared memory, and each CTA finishes a share of the tokens. The sums are integers:
+// no order of them changes a bit.
+#pragma once
+
+#include <cuda.h>
+
+#include "int8_kernels.cuh"
+
+namespace nvfp4 {
+
+constexpr int kInt8Threads = 192;
+constexpr int kInt8WeightBytes = 128 * 128;  // a stage's rows of B
+constexpr int kInt8MaxStages = 12;
+constexpr int kInt8MaxExperts = 1024;
+constexpr int kInt8Band = 8;  // token tiles that are walked together, channel tile by channel tile
+
+struct Int8TileParams {
+  CUtensorMap map_b;       // [experts][2 if gated][n][k], box 128 (gated: 2 x 16) rows of 128 bytes
+  CUtensorMap map_a;       // [rows][k], box of a whole tile's tokens (a pair: of half of them)
+  CUtensorMap map_a_part;  // the same with a box of 32 (a pair: 16) rows
+  const float* a_scales;
+  const float* b_scales;
+  const float* bias;
+  const int* offsets;
+  void* d;
+  long long ldd;
+  int rows, n, k, experts;
+  int out_kind;
+  int tile_tokens;  // 32, 64, 128 or 256
+  int stages;
+  int split;
+};
+
+// Set to a role's code when it abandons a wait; read and cleared by nvfp4_int8_status.
+__device__ int g_int8_status;
+constexpr int kInt8ProducerTimeout = 1, kInt8MmaInputTimeout = 2, kInt8MmaAccumTimeout = 3,
+              kInt8EpilogueTimeout = 4;
+
+__device__ __forceinline__ void int8_give_up(volatile int* abort_flag, int code) {
+  *abort_flag = 1;
+  atomicCAS(&g_int8_status, 0, code);
+}
+
+// D[tmem] (+)= A[smem] B[smem]^T, signed bytes, 32-bit integer sums, K = 32.
+template <int CTAS>
+__device__ __forceinline__ void tc_mma_i8(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b,
+                                          uint32_t idesc, uint32_t accumulate) {
+  if constexpr (CTAS == 1) {
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t"
+        "}" ::"r"(tmem_d),
+        "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+        : "memory");
+  } else {
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t"
+        "}" ::"r"(tmem_d),
+        "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+        : "memory");
+  }
+}
+
+// Instruction descriptor of kind::i8: 32-bit integer D (2 in bits 4-5), signed A and B (1 in bits
+// 7-9 and 10-12), K-major both, N and M in units of 8 and 16.
+__host__ __device__ constexpr uint32_t i8_instr_desc(uint32_t m, uint32_t n) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) | ((m >> 4) << 24);
+}
+
+// Tiled copies into this CTA's shared memory; `bar` is this CTA's barrier, or with a pair the
+// leader's (a shared::cluster address).
+template <int CTAS>
+__device__ __forceinline__ void tma_rows(uint32_t dst, const void* map, uint32_t bar, int k, int row) {
+  if constexpr (CTAS == 1) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, "
+        "%4}], [%2];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(k), "r"(row)
+        : "memory");
+  } else {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(k), "r"(row)
+        : "memory");
+  }
+}
+
+template <int CTAS>
+__device__ __forceinline__ void tma_weights(uint32_t dst, const void* map, uint32_t bar, int k,
+                                            int channel, int expert) {
+  if constexpr (CTAS == 1) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, "
+        "%4, %5, %6}], [%2];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(k), "r"(channel), "r"(0), "r"(expert)
+        : "memory");
+  } else {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(k), "r"(channel), "r"(0), "r"(expert)
+        : "memory");
+  }
+}
+
+template <int CTAS>
+__device__ __forceinline__ void int8_commit(uint32_t bar) {
+  if constexpr (CTAS == 1) {
+    tc_commit(bar);
+  } else {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
+        "[%0], %1;" ::"r"(bar),
+        "h"(static_cast<uint16_t>(3))
+        : "memory");
+  }
+}
+
+__device__ __forceinline__ int ld_cluster_s32(uint32_t addr) {
+  int v;
+  asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+struct Int8Tile {
+  int expert;
+  int m0;      // first token (row of A)
+  int tokens;  // tokens of the tile, at most tile_tokens
+  int columns; // tokens rounded up to the MMA's granularity of 32
+  int n_tile;
+};
+
+// Stores `v` (token column values of this lane's channel) for tokens m, m + 1, ... while they are
+// below `count`.
+template <typename T, int COLUMNS>
+__device__ __forceinline__ void store_columns(T* d, long long step, const float (&v)[COLUMNS], int count) {
+  if (count >= COLUMNS) {
+#pragma unroll
+    for (int i = 0; i < COLUMNS; ++i) {
+      *d = from_float<T>(v[i]);
+      d += step;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < COLUMNS; ++i) {
+      if (i < count) *d = from_float<T>(v[i]);
+      d += step;
+    }
+  }
+}
+
+template <int CTAS, bool GATED>
+__global__ void __launch_bounds__(kInt8Threads, 1)
+int8_tile_kernel(const __grid_constant__ Int8TileParams p) {
+  constexpr int kChannels = GATED ? 64 : 128;  // output channels of a CTA
+  extern __shared__ uint8_t dyn_smem[];
+  __shared__ alignas(8) uint64_t bar_full[kInt8MaxStages];
+  __shared__ alignas(8) uint64_t bar_empty[kInt8MaxStages];
+  __shared__ alignas(8) uint64_t bar_acc_full[2];
+  __shared__ alignas(8) uint64_t bar_acc_empty[2];
+  __shared__ alignas(16) float scale_stage[4][32];
+  __shared__ int tiles_before[kInt8MaxExperts + 1];  // token tiles of the experts before
+  __shared__ int first_row[kInt8MaxExperts + 1];
+  __shared__ uint32_t tmem_base_slot;
+  __shared__ int abort_flag;
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const uint32_t smem_base = (smem_u32(dyn_smem) + 1023u) & ~1023u;
+  const uint32_t rank = (CTAS == 2 || p.split > 1) ? cluster_cta_rank() : 0u;
+  const bool leader = CTAS == 1 || rank == 0;
+  const int tile_tokens = p.tile_tokens;
+  const int stages = p.stages;
+  const uint32_t stage_bytes = kInt8WeightBytes + static_cast<uint32_t>(tile_tokens / CTAS) * 128u;
+  const uint32_t tmem_cols = p.split > 1 ? tile_tokens : 2 * tile_tokens;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < stages; ++s) {
+      mbar_init(smem_u32(&bar_full[s]), 1);
+      mbar_init(smem_u32(&bar_empty[s]), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(&bar_acc_full[i]), 1);
+      mbar_init(smem_u32(&bar_acc_empty[i]), 4 * CTAS);
+    }
+    abort_flag = 0;
+    mbar_fence_init();
+  }
+  if (warp == 1) {
+    if constexpr (CTAS == 1) {
+      tmem_alloc(smem_u32(&tmem_base_slot), tmem_cols);
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                       smem_u32(&tmem_base_slot)),
+                   "r"(tmem_cols)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+  }
+  grid_dependency_wait();
+  grid_launch_dependents();
+  if (warp == 0) {
+    // First rows: the offsets cut to [0, rows], and where they decrease their running maximum, so
+    // that no value of theirs makes groups overlap or reach outside. Then a prefix over the
+    // experts' token tiles.
+    int before = 0, last_row = 0;
+    for (int e0 = 0; e0 < p.experts; e0 += 32) {
+      const int e = e0 + lane;
+      int row = e < p.experts ? (p.offsets != nullptr ? __ldg(p.offsets + e) : 0) : 0;
+      int next = e < p.experts ? (p.offsets != nullptr ? __ldg(p.offsets + e + 1) : p.rows) : 0;
+      row = min(max(row, last_row), p.rows);
+      next = min(max(next, row), p.rows);
+#pragma unroll
+      for (int d = 1; d < 32; d *= 2) {
+        const int other = __shfl_up_sync(0xFFFFFFFFu, next, d);
+        if (lane >= d) next = max(next, other);
+      }
+      const int previous = __shfl_up_sync(0xFFFFFFFFu, next, 1);
+      row = lane == 0 ? row : previous;
+      int tiles = e < p.experts ? (next - row + tile_tokens - 1) / tile_tokens : 0;
+#pragma unroll
+      for (int d = 1; d < 32; d *= 2) {
+        const int other = __shfl_up_sync(0xFFFFFFFFu, tiles, d);
+        if (lane >= d) tiles += other;
+      }
+      if (e == 0) first_row[0] = row;
+      if (e < p.experts) {
+        first_row[e + 1] = next;
+        tiles_before[e + 1] = before + tiles;
+      }
+      before += __shfl_sync(0xFFFFFFFFu, tiles, 31);
+      last_row = __shfl_sync(0xFFFFFFFFu, next, 31);
+    }
+    if (lane == 0) tiles_before[0] = 0;
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  if (CTAS == 2) cluster_sync_all();  // the peer's barriers and tensor memory exist
+  tc_fence_after_sync();
+  const uint32_t tmem_base = tmem_base_slot;
+  volatile int* abort_ptr = &abort_flag;
+
+  const int m_tiles = tiles_before[p.experts];
+  const int n_tiles = (p.n + kChannels * CTAS - 1) / (kChannels * CTAS);
+  const long long tiles = static_cast<long long>(m_tiles) * n_tiles;
+  const int group = p.split > 1 ? p.split : CTAS;  // CTAs that share a tile
+  const long long first_tile = blockIdx.x / group;
+  const long long step = gridDim.x / group;
+  const int k_tiles = (p.k + 127) / 128;
+  const int kt0 = p.split > 1 ? static_cast<int>(rank) * k_tiles / p.split : 0;
+  const int kt1 = p.split > 1 ? (static_cast<int>(rank) + 1) * k_tiles / p.split : k_tiles;
+
+  bool partials_written = false;  // a split tile's epilogue has passed the cluster's first barrier
+
+  auto decode = [&](long long t) {
+    Int8Tile tile;
+    const long long band_tiles = static_cast<long long>(kInt8Band) * n_tiles;
+    const int band = static_cast<int>(t / band_tiles);
+    const int in_band = static_cast<int>(t - band * band_tiles);
+    const int height = min(kInt8Band, m_tiles - band * kInt8Band);
+    const int m_tile = band * kInt8Band + in_band % height;
+    tile.n_tile = in_band / height;
+    // The last expert whose first tile is not behind m_tile, and that has tiles.
+    int lo = 0, hi = p.experts;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (tiles_before[mid] <= m_tile) lo = mid; else hi = mid;
+    }
+    tile.expert = lo;
+    tile.m0 = first_row[lo] + (m_tile - tiles_before[lo]) * tile_tokens;
+    tile.tokens = min(tile_tokens, first_row[lo + 1] - tile.m0);
+    tile.columns = (tile.tokens + 31) & ~31;
+    return tile;
+  };
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------ producer
+    if (elect_one()) {
+      prefetch_tensormap(&p.map_b);
+      prefetch_tensormap(&p.map_a);
+      prefetch_tensormap(&p.map_a_part);
+    }
+    const uint32_t full0 = CTAS == 1 ? smem_u32(&bar_full[0])
+                                     : cluster_map_shared(smem_u32(&bar_full[0]), 0);
+    const uint32_t empty0 = smem_u32(&bar_empty[0]);
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (long long t = first_tile; ok && t < tiles; t += step) {
+      const Int8Tile tile = decode(t);
+      const int channel0 = (tile.n_tile * CTAS + static_cast<int>(CTAS == 2 ? rank : 0)) * kChannels;
+      const int share = tile.columns / CTAS;  // tokens this CTA loads
+      const int token0 = tile.m0 + static_cast<int>(CTAS == 2 ? rank : 0) * share;
+      const uint32_t bytes = kInt8WeightBytes + static_cast<uint32_t>(share) * 128u;
+      for (int kt = kt0; kt < kt1; ++kt) {
+        if (!mbar_wait(empty0 + 8 * stage, phase ^ 1u, abort_ptr)) {
+          int8_give_up(abort_ptr, kInt8ProducerTimeout);
+          ok = false;
+          break;
+        }
+        const uint32_t w_dst = smem_base + stage * stage_bytes;
+        const uint32_t t_dst = w_dst + kInt8WeightBytes;
+        const uint32_t bar = full0 + 8 * stage;
+        if (elect_one()) {
+          if (leader) mbar_expect_tx(smem_u32(&bar_full[stage]), CTAS * bytes);
+          if constexpr (GATED) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              tma_weights<CTAS>(w_dst + 4096 * j, &p.map_b, bar, kt * 128, channel0 + 16 * j, tile.expert);
+            }
+          } else {
+            tma_weights<CTAS>(w_dst, &p.map_b, bar, kt * 128, channel0, tile.expert);
+          }
+          if (tile.columns == tile_tokens) {
+            tma_rows<CTAS>(t_dst, &p.map_a, bar, kt * 128, token0);
+          } else {
+            for (int c = 0; c < share; c += 32 / CTAS) {
+              tma_rows<CTAS>(t_dst + c * 128, &p.map_a_part, bar, kt * 128, token0 + c);
+            }
+          }
+        }
+        __syncwarp();
+        if (++stage == stages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+    }
+    if (!ok || *abort_ptr != 0) {
+      // Copies may still be on their way into this CTA's memory: let them land.
+      for (int i = 0; i < 64; ++i) __nanosleep(1000);
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ MMA issuer
+    if (leader) {
+      constexpr uint32_t kHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+      const uint32_t lo0 = ((smem_base >> 4) & 0x3FFFu) | (1u << 16);
+      const uint32_t full0 = smem_u32(&bar_full[0]);
+      const uint32_t empty0 = smem_u32(&bar_empty[0]);
+      int stage = 0;
+      uint32_t phase = 0;
+      uint32_t acc = 0, acc_phase = 0;
+      bool ok = true;
+      for (long long t = first_tile; ok && t < tiles; t += step) {
+        const Int8Tile tile = decode(t);
+        const uint32_t idesc = i8_instr_desc(128 * CTAS, static_cast<uint32_t>(tile.columns));
+        if (!mbar_wait(smem_u32(&bar_acc_empty[acc]), acc_phase ^ 1u, abort_ptr)) {
+          int8_give_up(abort_ptr, kInt8MmaAccumTimeout);
+          break;
+        }
+        tc_fence_after_sync();
+        const uint32_t d = tmem_base + acc * tile_tokens;
+        uint32_t accumulate = 0;
+        for (int kt = kt0; kt < kt1; ++kt) {
+          if (!mbar_wait(full0 + 8 * stage, phase, abort_ptr)) {
+            int8_give_up(abort_ptr, kInt8MmaInputTimeout);
+            ok = false;
+            break;
+          }
+          tc_fence_after_sync();
+          const uint32_t lo_w = lo0 + ((stage * stage_bytes) >> 4);
+          const uint32_t lo_t = lo_w + (kInt8WeightBytes >> 4);
+          if (elect_one()) {
+            // The last stage's k beyond the depth is zero in both operands: not multiplied.
+            const int mmas = min(4, (p.k - kt * 128 + 31) / 32);
+            for (int j = 0; j < mmas; ++j) {
+              tc_mma_i8<CTAS>(d, pack_desc(lo_w + 2 * j, kHi), pack_desc(lo_t + 2 * j, kHi), idesc,
+                              j > 0 ? 1u : accumulate);
+            }
+            int8_commit<CTAS>(empty0 + 8 * stage);
+          }
+          __syncwarp();
+          accumulate = 1;
+          if (++stage == stages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+        if (!ok) break;
+        if (elect_one()) int8_commit<CTAS>(smem_u32(&bar_acc_full[acc]));
+        __syncwarp();
+        acc ^= 1u;
+        if (acc == 0) acc_phase ^= 1u;
+      }
+    }
+  } else {
+    // ------------------------------------------------------------------ epilogue
+    const int quarter = warp & 3;
+    float* sa_stage = scale_stage[quarter];
+    const uint32_t leader_acc_empty0 = CTAS == 1 ? smem_u32(&bar_acc_empty[0])
+                                                 : cluster_map_shared(smem_u32(&bar_acc_empty[0]), 0);
+    uint32_t acc = 0, acc_phase = 0;
+    for (long long t = first_tile; t < tiles; t += step) {
+      const Int8Tile tile = decode(t);
+      // This lane's row of B: its channel in D, and its place among the scales.
+      const int channel0 = (tile.n_tile * CTAS + static_cast<int>(CTAS == 2 ? rank : 0)) * kChannels;
+      const int channel = GATED ? channel0 + quarter * 16 + (lane & 15) : channel0 + quarter * 32 + lane;
+      const bool live = channel < p.n;
+      const int width = GATED ? 2 * p.n : p.n;
+      const int row = GATED && lane >= 16 ? p.n + channel : channel;
+      const float sb = live ? __ldg(p.b_scales + static_cast<long long>(tile.expert) * width + row) : 0.0f;
+      const float bias = live && p.bias != nullptr ? __ldg(p.bias + row) : 0.0f;
+      if (!mbar_wait(smem_u32(&bar_acc_full[acc]), acc_phase, abort_ptr)) {
+        int8_give_up(abort_ptr, kInt8EpilogueTimeout);
+        break;
+      }
+      tc_fence_after_sync();
+      const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + acc * tile_tokens;
+      int c_begin = 0, c_end = tile.columns;
+      if (p.split > 1) {
+        // Partial sums to shared memory (the stages are free: every MMA that read them is done),
+        // [token][channel row]; after the cluster's barrier each CTA adds up its share of tokens.
+        for (int c = 0; c < tile.columns; c += 32) {
+          uint32_t r[32];
+          tmem_load_32(taddr + c, r);
+          tmem_load_wait();
+          const uint32_t to = smem_base + static_cast<uint32_t>(c * 128 + quarter * 32 + lane) * 4u;
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            asm volatile("st.shared.b32 [%0], %1;" ::"r"(to + i * 512), "r"(r[i]) : "memory");
+          }
+        }
+        cluster_sync_all();
+        partials_written = true;
+        c_begin = tile.columns * static_cast<int>(rank) / p.split;
+        c_end = tile.columns * (static_cast<int>(rank) + 1) / p.split;
+      }
+      for (int c = c_begin; c < min(c_end, tile.tokens); c += 32) {
+        const int count = min(min(c_end, tile.tokens) - c, 32);
+        sa_stage[lane] = lane < count ? __ldg(p.a_scales + tile.m0 + c + lane) : 0.0f;
+        uint32_t r[32];
+        if (p.split > 1) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) r[i] = 0;
+          for (int s = 0; s < p.split; ++s) {
+            const uint32_t from = cluster_map_shared(
+                smem_base + static_cast<uint32_t>(c * 128 + quarter * 32 + lane) * 4u, s);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              if (i < count) r[i] += static_cast<uint32_t>(ld_cluster_s32(from + i * 512));
+            }
+          }
+        } else {
+          tmem_load_32(taddr + c, r);
+          tmem_load_wait();
+        }
+        __syncwarp();
+        float v[32];
+#pragma unroll
+        for (int i = 0; i < 32; i += 4) {
+          const float4 sa = *reinterpret_cast<const float4*>(sa_stage + i);
+          const float s[4] = {sa.x, sa.y, sa.z, sa.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            v[i + j] = __fmul_rn(__fmul_rn(static_cast<float>(static_cast<int>(r[i + j])), s[j]), sb);
+          }
+        }
+        if (p.bias != nullptr) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = __fadd_rn(v[i], bias);
+        }
+        __syncwarp();
+        if constexpr (GATED) {
+          // Of tokens 2i and 2i + 1 the gate lanes finish the first, the up lanes the second.
+          float y[16];
+          const bool up_lane = lane >= 16;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float mine = up_lane ? v[2 * i + 1] : v[2 * i];
+            const float other = __shfl_xor_sync(0xFFFFFFFFu, up_lane ? v[2 * i] : v[2 * i + 1], 16);
+            y[i] = up_lane ? silu(other) * mine : silu(mine) * other;
+          }
+          const int parity = up_lane ? 1 : 0;
+          const long long first = (tile.m0 + c + parity) * p.ldd + channel;
+          const int mine = live ? (count - parity + 1) / 2 : 0;
+          if (p.out_kind == 0) {
+            store_columns(static_cast<__half*>(p.d) + first, 2 * p.ldd, y, mine);
+          } else if (p.out_kind == 1) {
+            store_columns(static_cast<float*>(p.d) + first, 2 * p.ldd, y, mine);
+          } else {
+            store_columns(static_cast<__nv_bfloat16*>(p.d) + first, 2 * p.ldd, y, mine);
+          }
+        } else {
+          const long long first = (tile.m0 + c) * p.ldd + channel;
+          const int mine = live ? count : 0;
+          if (p.out_kind == 0) {
+            store_columns(static_cast<__half*>(p.d) + first, p.ldd, v, mine);
+          } else if (p.out_kind == 1) {
+            store_columns(static_cast<float*>(p.d) + first, p.ldd, v, mine);
+          } else {
+            store_columns(static_cast<__nv_bfloat16*>(p.d) + first, p.ldd, v, mine);
+          }
+        }
+      }
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) {
+        if constexpr (CTAS == 1) {
+          mbar_arrive(leader_acc_empty0 + 8 * acc);
+        } else {
+          mbar_arrive_peer(leader_acc_empty0 + 8 * acc);
+        }
+      }
+      acc ^= 1u;
+      if (acc == 0) acc_phase ^= 1u;
+    }
+  }
+
+  tc_fence_before_sync();
+  __syncwarp();
+  if (p.split > 1) {
+    // Two phases of the cluster's barrier, in every thread: the partial sums are written; they are
+    // read. An epilogue warp with a tile has passed the first above.
+    if (!partials_written) cluster_sync_all();
+    cluster_sync_all();
+  }
+  __syncthreads();
+  if (CTAS == 2) cluster_sync_all();  // neither CTA frees tensor memory while the pair is in use
+  if (warp == 1) {
+    tc_fence_after_sync();
+    __syncwarp();
+    if constexpr (CTAS == 1) {
+      tmem_dealloc(tmem_base, tmem_cols);
+    } else {
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base),
+                   "r"(tmem_cols)
+                   : "memory");
+    }
+  }
+}
+
+}  // namespace nvfp4

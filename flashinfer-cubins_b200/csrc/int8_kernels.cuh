@@ -211,112 +211,8 @@ __global__ void __launch_bounds__(kRowThreads) residual_norm_kernel(const NormPa
 // Products
 // ---------------------------------------------------------------------------
 
-struct Int8GemmParams {
-  const int8_t* a;  // [rows][k]
-  const int8_t* b;  // [experts][width][k]; width = n, or 2 n with a gate (gate rows, then up rows)
-  const float* a_scales;
-  const float* b_scales;  // [experts][width]
-  const float* bias;      // [width] or null
-  const int* offsets;     // [experts + 1] or null: one group of all rows
-  void* d;                // [rows][n]
-  long long lda, ldb, expert_stride, ldd;
-  int rows, n, k, experts;
-  int out_kind;  // NVFP4_OUT_F16, _F32, _BF16
-};
-
 // x * sigmoid(x).
 __device__ __forceinline__ float silu(float x) { return x * __fdividef(1.0f, 1.0f + __expf(-x)); }
-
-__device__ __forceinline__ void store_out(void* d, long long i, int out_kind, float v) {
-  if (out_kind == 0) {
-    static_cast<__half*>(d)[i] = from_float<__half>(v);
-  } else if (out_kind == 1) {
-    static_cast<float*>(d)[i] = v;
-  } else {
-    static_cast<__nv_bfloat16*>(d)[i] = from_float<__nv_bfloat16>(v);
-  }
-}
-
-// Rows [lo, hi) of expert e, whatever the offsets hold: never outside [0, rows).
-__device__ __forceinline__ void expert_rows(const int* offsets, int e, int rows, int* lo, int* hi) {
-  if (offsets == nullptr) {
-    *lo = 0;
-    *hi = rows;
-    return;
-  }
-  *lo = min(max(offsets[e], 0), rows);
-  *hi = min(max(offsets[e + 1], *lo), rows);
-}
-
-// Four bytes of a row from column c on, zero from column k on.
-__device__ __forceinline__ int load_word(const int8_t* row, int c, int k) {
-  int w = *reinterpret_cast<const int*>(row + c);
-  if (c + 4 > k) w &= (1 << (8 * (k - c))) - 1;
-  return w;
-}
-
-constexpr int kTile = 64;  // tokens and channels of a tile
-
-template <bool GATED>
-__global__ void __launch_bounds__(256) int8_gemm_kernel(const Int8GemmParams p) {
-  constexpr int HALVES = GATED ? 2 : 1;
-  __shared__ int as[kTile][17], bs[HALVES][kTile][17];
-  int e = 0, lo = 0, hi = 0;
-  long long tile = blockIdx.y;
-  for (; e < p.experts; ++e) {
-    expert_rows(p.offsets, e, p.rows, &lo, &hi);
-    const int tiles = (hi - lo + kTile - 1) / kTile;
-    if (tile < tiles) break;
-    tile -= tiles;
-  }
-  if (e == p.experts) return;
-  const int m0 = lo + static_cast<int>(tile) * kTile, n0 = blockIdx.x * kTile;
-  const int8_t* b = p.b + e * p.expert_stride;
-  const float* b_scales = p.b_scales + static_cast<long long>(e) * HALVES * p.n;
-  const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
-  int acc[HALVES][4][4] = {};
-  for (int k0 = 0; k0 < p.k; k0 += 64) {
-    for (int i = threadIdx.x; i < kTile * 16; i += 256) {
-      const int r = i / 16, c = k0 + 4 * (i % 16);
-      as[r][i % 16] = m0 + r < hi && c < p.k ? load_word(p.a + (m0 + r) * p.lda, c, p.k) : 0;
-      for (int h = 0; h < HALVES; ++h) {
-        bs[h][r][i % 16] = n0 + r < p.n && c < p.k
-            ? load_word(b + (static_cast<long long>(h) * p.n + n0 + r) * p.ldb, c, p.k) : 0;
-      }
-    }
-    __syncthreads();
-    for (int j = 0; j < 16; ++j) {
-      for (int h = 0; h < HALVES; ++h) {
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-#pragma unroll
-          for (int v = 0; v < 4; ++v) {
-            acc[h][u][v] = __dp4a(as[ty + 16 * u][j], bs[h][tx + 16 * v][j], acc[h][u][v]);
-          }
-        }
-      }
-    }
-    __syncthreads();
-  }
-#pragma unroll
-  for (int u = 0; u < 4; ++u) {
-    const int m = m0 + ty + 16 * u;
-    if (m >= hi) continue;
-    const float sa = p.a_scales[m];
-#pragma unroll
-    for (int v = 0; v < 4; ++v) {
-      const int n = n0 + tx + 16 * v;
-      if (n >= p.n) continue;
-      float y[HALVES];
-#pragma unroll
-      for (int h = 0; h < HALVES; ++h) {
-        y[h] = static_cast<float>(acc[h][u][v]) * sa * b_scales[h * p.n + n];
-        if (p.bias != nullptr) y[h] += p.bias[h * p.n + n];
-      }
-      store_out(p.d, m * p.ldd + n, p.out_kind, GATED ? silu(y[0]) * y[HALVES - 1] : y[0]);
-    }
-  }
-}
 
 // Routing of pairs to unpadded groups: offsets[e] = number of pairs of the experts before e
 // (offsets[experts]: of all), and a cursor per expert that starts there.

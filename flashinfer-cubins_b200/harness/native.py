@@ -168,6 +168,7 @@ _PROTOTYPES = {
         ctypes.c_int, [_P, ctypes.c_longlong, _P, ctypes.c_longlong, ctypes.c_longlong, _P, _P, _P,
                        _P, ctypes.c_longlong] + [ctypes.c_int] * 6 + [_P],
     ),
+    "nvfp4_int8_status": (ctypes.c_int, [_P, ctypes.POINTER(ctypes.c_int)]),
     "nvfp4_int8_quantize": (
         ctypes.c_int, [_P, ctypes.c_int, ctypes.c_longlong, _P, ctypes.c_int, ctypes.c_int,
                        ctypes.c_int, _P, ctypes.c_longlong, _P, _P],

@@ -383,11 +383,17 @@ int nvfp4_int8_gemm(const void* a, long long lda, const void* b, long long ldb,
 /* The same with rows offsets[e] .. offsets[e + 1] of A, a_scales and D (device, `experts` + 1 ints
  * that do not decrease) multiplied by expert e's weights, `expert_stride` bytes after the previous
  * expert's; b_scales [experts][n or 2 n]. Rows of D that no expert owns are left as they were.
- * Offsets are cut to [0, rows]: no value of theirs reaches outside the buffers. */
+ * Offsets are cut to [0, rows], and one below those before it counts as the largest of them: no
+ * value of theirs reaches outside the buffers or makes two experts share a row. */
 int nvfp4_int8_group_gemm(const void* a, long long lda, const void* b, long long ldb,
                           long long expert_stride, const float* a_scales, const float* b_scales,
                           const int* offsets, void* d, long long ldd, int experts, int rows, int n,
                           int k, int out_kind, int gated, void* stream);
+
+/* Synchronises `stream` and reads the status word that the products of the current device share
+ * (0 = ok): NVFP4_E_DEVICE_TIMEOUT if a kernel abandoned a bounded wait since the last call, whose
+ * output is then undefined. Clears the word. */
+int nvfp4_int8_status(void* stream, int* status);
 
 /* Rows of x (FP32, BF16 or FP16, ldx elements apart) -> INT8 codes q (ldq bytes apart) and a scale
  * for each: scale = max |x| / 127 and code = x / scale to the nearest integer, ties to even, both
