@@ -190,11 +190,89 @@ int launch_product(const Product& q, void* stream) {
   return 0;
 }
 
-template <typename In>
-void launch_quantize(int blocks, cudaStream_t s, const void* x, long long ldx, const int* source,
-                     int rows, int tokens, int k, void* q, long long ldq, float* scales) {
-  int8_quantize_kernel<In><<<blocks, kRowThreads, 0, s>>>(
-      static_cast<const In*>(x), ldx, source, rows, tokens, k, static_cast<int8_t*>(q), ldq, scales);
+// How rows of `width` elements lie over threads. A warp to a row up to 1,024 elements, where there
+// are rows enough; else a CTA. In pieces of eight: few threads with much work where there are many
+// rows (`elements` a thread: fewer, and the fixed cost of a row's reductions shows), many threads
+// where there are too few to fill the SMs (a row's latency is what counts then). One at a time: 8
+// elements a thread, or what 1,024 threads need.
+struct RowGrid {
+  int elements, threads, blocks;
+  bool warp;
+};
+
+constexpr int kMaxRegisterRow = 32768;
+
+RowGrid row_grid(int rows, int width, int p, int elements) {
+  RowGrid g{};
+  g.warp = width <= 1024 && rows > host_sm_count();
+  if (g.warp) {
+    g.elements = width <= 256 ? 8 : 32;
+    g.threads = 32 * kWarpRows;
+    g.blocks = (rows + kWarpRows - 1) / kWarpRows;
+    return g;
+  }
+  g.elements = p == 8 && rows > 2 * host_sm_count() ? elements : 8;
+  while ((width + g.elements - 1) / g.elements > 1024) g.elements *= 2;
+  g.threads = ((width + g.elements - 1) / g.elements + 31) / 32 * 32;
+  if (p == 1) g.threads = g.threads <= 128 ? 128 : g.threads <= 256 ? 256 : g.threads <= 512 ? 512 : 1024;
+  g.blocks = rows;
+  return g;
+}
+
+template <bool WIDE, int P>
+void launch_quantize(const RowGrid& g, cudaStream_t s, const QuantizeParams& p) {
+  constexpr int kWarps = 32 * kWarpRows;
+  void (*kernel)(QuantizeParams);
+  if (g.warp) {
+    kernel = g.elements == 8 ? int8_quantize_kernel<WIDE, P, 8 / P, kWarps, true>
+                             : int8_quantize_kernel<WIDE, P, 32 / P, kWarps, true>;
+  } else if (P == 1 && g.threads < 1024) {
+    kernel = g.threads == 128   ? int8_quantize_kernel<WIDE, 1, 8, 128, false>
+             : g.threads == 256 ? int8_quantize_kernel<WIDE, 1, 8, 256, false>
+                                : int8_quantize_kernel<WIDE, 1, 8, 512, false>;
+  } else {
+    kernel = g.elements == 8    ? int8_quantize_kernel<WIDE, P, 8 / P, 1024, false>
+             : g.elements == 16 ? int8_quantize_kernel<WIDE, P, 16 / P, 1024, false>
+             : g.threads <= 512 ? int8_quantize_kernel<WIDE, P, 32 / P, 512, false>
+                                : int8_quantize_kernel<WIDE, P, 32 / P, 1024, false>;
+  }
+  kernel<<<g.blocks, g.threads, 0, s>>>(p);
+}
+
+template <bool X_WIDE, bool R_WIDE, int P>
+void launch_norm(const RowGrid& g, cudaStream_t s, const NormParams& p) {
+  constexpr int kWarps = 32 * kWarpRows;
+  void (*kernel)(NormParams);
+  if (g.warp) {
+    kernel = g.elements == 8 ? residual_norm_kernel<X_WIDE, R_WIDE, P, 8 / P, kWarps, true>
+                             : residual_norm_kernel<X_WIDE, R_WIDE, P, 32 / P, kWarps, true>;
+  } else if (P == 1 && g.threads < 1024) {
+    kernel = g.threads == 128   ? residual_norm_kernel<X_WIDE, R_WIDE, 1, 8, 128, false>
+             : g.threads == 256 ? residual_norm_kernel<X_WIDE, R_WIDE, 1, 8, 256, false>
+                                : residual_norm_kernel<X_WIDE, R_WIDE, 1, 8, 512, false>;
+  } else {
+    kernel = g.elements == 8    ? residual_norm_kernel<X_WIDE, R_WIDE, P, 8 / P, 1024, false>
+             : g.elements == 32 ? residual_norm_kernel<X_WIDE, R_WIDE, P, 32 / P, 1024, false>
+             : g.threads <= 512 ? residual_norm_kernel<X_WIDE, R_WIDE, P, 16 / P, 512, false>
+                                : residual_norm_kernel<X_WIDE, R_WIDE, P, 16 / P, 1024, false>;
+  }
+  kernel<<<g.blocks, g.threads, 0, s>>>(p);
+}
+
+template <int P>
+void launch_norm(const RowGrid& g, cudaStream_t s, const NormParams& p) {
+  const bool wide_r = p.residual != nullptr && p.residual_kind == NVFP4_IN_F32;
+  if (p.x_kind == NVFP4_IN_F32) {
+    if (wide_r) launch_norm<true, true, P>(g, s, p); else launch_norm<true, false, P>(g, s, p);
+  } else {
+    if (wide_r) launch_norm<false, true, P>(g, s, p); else launch_norm<false, false, P>(g, s, p);
+  }
+}
+
+// Whether rows of `bytes`-sized elements, `pitch` elements apart, all start on a multiple of eight
+// elements.
+bool rows_in_eights(const void* p, long long pitch, int bytes, int rows) {
+  return aligned(p, 8 * bytes) && (rows <= 1 || pitch % 8 == 0);
 }
 
 }  // namespace
@@ -252,14 +330,17 @@ int nvfp4_int8_quantize(const void* x, int x_kind, long long ldx, const int* sou
   if (!aligned(x, kind_bytes(x_kind)) || !aligned(scales, 4) || !aligned(source_rows, 4)) {
     return fail(NVFP4_E_MISALIGNED, "misaligned operand address");
   }
-  const int blocks = std::min(rows, 8 * host_sm_count());
+  const QuantizeParams p{x, source_rows, static_cast<int8_t*>(q), scales, ldx, ldq,
+                         rows, tokens, k, x_kind};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (x_kind == NVFP4_IN_F32) {
-    launch_quantize<float>(blocks, s, x, ldx, source_rows, rows, tokens, k, q, ldq, scales);
-  } else if (x_kind == NVFP4_IN_BF16) {
-    launch_quantize<__nv_bfloat16>(blocks, s, x, ldx, source_rows, rows, tokens, k, q, ldq, scales);
+  if (k > kMaxRegisterRow) {
+    int8_quantize_long_kernel<<<rows, 1024, 0, s>>>(p);
+  } else if (rows_in_eights(x, ldx, kind_bytes(x_kind), tokens) && rows_in_eights(q, ldq, 1, rows)) {
+    const RowGrid g = row_grid(rows, k, 8, 32);
+    if (x_kind == NVFP4_IN_F32) launch_quantize<true, 8>(g, s, p); else launch_quantize<false, 8>(g, s, p);
   } else {
-    launch_quantize<__half>(blocks, s, x, ldx, source_rows, rows, tokens, k, q, ldq, scales);
+    const RowGrid g = row_grid(rows, k, 1, 32);
+    if (x_kind == NVFP4_IN_F32) launch_quantize<true, 1>(g, s, p); else launch_quantize<false, 1>(g, s, p);
   }
   CUDA_TRY(cudaGetLastError());
   return 0;
@@ -323,14 +404,21 @@ int nvfp4_residual_norm(const void* x, int x_kind, long long ldx, const void* re
   p.tokens_per_gate = gate != nullptr ? tokens / gates : 1;
   p.residual_scale = residual_scale;
   p.eps = eps;
+  p.inverse_hidden = 1.0 / hidden;
   p.x_kind = x_kind;
   p.residual_kind = residual_kind;
   p.y_kind = y_kind;
-  const size_t bytes = static_cast<size_t>(hidden) * sizeof(float);
-  CUDA_TRY(cudaFuncSetAttribute(residual_norm_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                kMaxHidden * static_cast<int>(sizeof(float))));
-  const int blocks = std::min(tokens, 8 * host_sm_count());
-  residual_norm_kernel<<<blocks, kRowThreads, bytes, static_cast<cudaStream_t>(stream)>>>(p);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int y_bytes = y_kind == NVFP4_NORM_CODES ? 1 : kind_bytes(y_kind);
+  const int r_bytes = static_cast<int>(residual_bytes);
+  if (rows_in_eights(x, ldx, kind_bytes(x_kind), tokens) && rows_in_eights(residual, ldres, r_bytes, tokens) &&
+      rows_in_eights(r, ldr, r_bytes, tokens) && rows_in_eights(post_weight, 0, 4, 1) &&
+      rows_in_eights(gate, hidden, 4, gates) &&
+      (next_weight == nullptr || (rows_in_eights(next_weight, 0, 4, 1) && rows_in_eights(y, ldy, y_bytes, tokens)))) {
+    launch_norm<8>(row_grid(tokens, hidden, 8, 16), s, p);
+  } else {
+    launch_norm<1>(row_grid(tokens, hidden, 1, 16), s, p);
+  }
   CUDA_TRY(cudaGetLastError());
   return 0;
 }

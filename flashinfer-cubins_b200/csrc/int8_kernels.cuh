@@ -46,69 +46,326 @@ __device__ __forceinline__ float row_scale(uint32_t amax_bits) {
   return __fdiv_rn(__uint_as_float(amax_bits), 127.0f);
 }
 
-// The code of v: the integer nearest to v / scale, ties to even, within +-127 (beyond them only
-// where the scale itself is so small that it was rounded).
+// The code of v: the integer nearest to the correctly rounded v / scale, ties to even, within
+// +-127 (beyond them only where the scale is subnormal and was rounded coarsely).
 __device__ __forceinline__ int row_code(float v, float scale) {
   const float q = rintf(__fdiv_rn(v, scale));
   return static_cast<int>(fminf(fmaxf(q, -127.0f), 127.0f));
 }
 
-// Whether the row has codes at all: not if it is zero (or its scale is), infinite or NaN.
-__device__ __forceinline__ bool row_has_codes(uint32_t amax_bits, float scale) {
-  return amax_bits < 0x7F800000u && scale > 0.0f;
+// How a row's codes are made.
+struct RowCodes {
+  float scale, inverse;
+  bool live;     // false: zero row (or scale), infinite or NaN: codes are zero
+  bool divide;   // the scale is subnormal: divide every value
+};
+
+__device__ __forceinline__ RowCodes row_codes(uint32_t amax_bits) {
+  RowCodes r;
+  r.scale = row_scale(amax_bits);
+  r.live = amax_bits < 0x7F800000u && r.scale > 0.0f;
+  r.divide = r.scale < 1.17549435e-38f;
+  r.inverse = __frcp_rn(r.scale);
+  return r;
 }
 
-template <int THREADS>
-__device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t* shared) {
-  v = __reduce_max_sync(0xFFFFFFFFu, v);
-  if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = v;
-  __syncthreads();
-  uint32_t all = 0;
+// Codes of values. A product with the reciprocal decides: it is within 1.5 steps of 2^-17 of the
+// quotient (|q| <= 127), so where it lies more than 2^-15 from the middle between two integers the
+// quotient, rounded, lies on the same side. Adding 1.5 * 2^23 rounds it to an integer (ties to even)
+// whose low byte is the code. Values nearer to a middle (one in 2^14) are divided. Dividing all of
+// them cost 94 us for 8192 x 7168 BF16 values, this 35.
+constexpr float kRoundBias = 12582912.0f;
+
+__device__ __forceinline__ bool near_middle(float off) { return off >= 0.5f - 0x1p-15f; }
+
+__device__ __forceinline__ uint2 eight_codes(const float (&v)[8], const RowCodes& row) {
+  if (!row.live) return make_uint2(0u, 0u);
+  const float2 inverse = make_float2(row.inverse, row.inverse), round = make_float2(kRoundBias, kRoundBias);
+  uint32_t b[8];
+  float off = 0.0f;
 #pragma unroll
-  for (int w = 0; w < THREADS / 32; ++w) all = max(all, shared[w]);
-  __syncthreads();
-  return all;
+  for (int i = 0; i < 8; i += 2) {
+    const float2 x = make_float2(v[i], v[i + 1]);
+    const float2 t = __ffma2_rn(x, inverse, round);                          // round + n
+    const float2 n = __ffma2_rn(t, make_float2(-1.0f, -1.0f), round);        // -n
+    const float2 d = __ffma2_rn(x, inverse, n);
+    off = fmaxf(fmaxf(off, fabsf(d.x)), fabsf(d.y));
+    b[i] = __float_as_uint(t.x);
+    b[i + 1] = __float_as_uint(t.y);
+  }
+  if (row.divide || near_middle(off)) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) b[i] = static_cast<uint32_t>(row_code(v[i], row.scale));
+  }
+  return make_uint2(
+      __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410),
+      __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410));
 }
 
-template <int THREADS>
-__device__ __forceinline__ double block_sum(double v, double* shared) {
+__device__ __forceinline__ int one_code(float v, const RowCodes& row) {
+  if (!row.live) return 0;
+  const float t = fmaf(v, row.inverse, kRoundBias);
+  const float off = fabsf(fmaf(v, row.inverse, kRoundBias - t));
+  if (row.divide || near_middle(off)) return row_code(v, row.scale);
+  return static_cast<int>(__float_as_uint(t));
+}
+
+// ---------------------------------------------------------------------------
+// Rows in registers
+// ---------------------------------------------------------------------------
+//
+// A row belongs to one warp (WARP: eight rows to a CTA, no barrier) or to one CTA, whose threads
+// hold N pieces of P neighbouring elements each, read once, every load issued before the first is
+// used. P = 8 where all rows start on a multiple of eight elements: 16-byte loads of 16-bit
+// elements, 32-byte ones of 32-bit elements (two 16-byte loads a lane, 32 bytes apart, took the L1
+// cache twice the cycles), and a last piece that may be short. P = 1 for any other start and pitch:
+// there the CTA has its full THREADS, so that a thread's elements lie constant distances apart and
+// an access needs no address of its own (8192 x 5121 norms: 319 us with computed addresses).
+
+__device__ __forceinline__ void load_32_bytes(const void* p, uint32_t (&w)[8]) {
+  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+               : "l"(p));
+}
+
+__device__ __forceinline__ void store_32_bytes(void* p, const float (&v)[8]) {
+  asm volatile("st.global.v8.f32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::"f"(v[0]), "f"(v[1]), "f"(v[2]),
+               "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]), "l"(p)
+               : "memory");
+}
+
+// P elements as they lie in memory.
+template <bool WIDE, int P>
+struct Raw {
+  static constexpr int kWords = WIDE ? P : (P + 1) / 2;
+  uint32_t w[kWords];
+};
+
+// Elements c .. c + P - 1 of a row of which `left` are there; zero beyond them.
+template <bool WIDE, int P>
+__device__ __forceinline__ Raw<WIDE, P> load_raw(const void* row, int c, int left) {
+  Raw<WIDE, P> r;
+  if constexpr (P == 1) {
+    r.w[0] = 0;
+    if (left > 0) {
+      if constexpr (WIDE) {
+        r.w[0] = static_cast<const uint32_t*>(row)[c];
+      } else {
+        r.w[0] = static_cast<const uint16_t*>(row)[c];
+      }
+    }
+  } else {
+    if (left >= 8) {
+      if constexpr (WIDE) {
+        load_32_bytes(static_cast<const float*>(row) + c, r.w);
+      } else {
+        const uint4 q = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(row) + c);
+        r.w[0] = q.x;
+        r.w[1] = q.y;
+        r.w[2] = q.z;
+        r.w[3] = q.w;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < Raw<WIDE, P>::kWords; ++i) r.w[i] = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (i < left) {
+          if constexpr (WIDE) {
+            r.w[i] = static_cast<const uint32_t*>(row)[c + i];
+          } else {
+            r.w[i / 2] |= static_cast<uint32_t>(static_cast<const uint16_t*>(row)[c + i]) << (16 * (i % 2));
+          }
+        }
+      }
+    }
+  }
+  return r;
+}
+
+// The values; `half`: 16-bit elements are FP16, else BF16.
+template <bool WIDE, int P>
+__device__ __forceinline__ void unpack(const Raw<WIDE, P>& r, bool half, float (&v)[P]) {
+  if constexpr (WIDE) {
+#pragma unroll
+    for (int i = 0; i < P; ++i) v[i] = __uint_as_float(r.w[i]);
+  } else if (half) {
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      v[i] = __half2float(__ushort_as_half(static_cast<unsigned short>(r.w[i / 2] >> (16 * (i % 2)))));
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      v[i] = __uint_as_float(i % 2 != 0 ? r.w[i / 2] & 0xFFFF0000u : r.w[i / 2] << 16);
+    }
+  }
+}
+
+// FP32 values of a vector over the row (weights, gates), zero beyond it.
+template <int P>
+__device__ __forceinline__ void load_weights(const float* row, int c, int left, float (&v)[P]) {
+  unpack<true, P>(load_raw<true, P>(row, c, left), false, v);
+}
+
+// Stores values of kind NVFP4_IN_*.
+template <int P>
+__device__ __forceinline__ void store_values(void* row, int c, int left, int kind, const float (&v)[P]) {
+  if (kind == 0) {
+    float* p = static_cast<float*>(row) + c;
+    if constexpr (P == 8) {
+      if (left >= 8) {
+        store_32_bytes(p, v);
+        return;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      if (i < left) p[i] = v[i];
+    }
+    return;
+  }
+  uint32_t w[(P + 1) / 2];
+#pragma unroll
+  for (int i = 0; i < (P + 1) / 2; ++i) {
+    const float low = v[2 * i], high = 2 * i + 1 < P ? v[(2 * i + 1) % P] : 0.0f;
+    if (kind == 1) {
+      const __nv_bfloat162 b = __floats2bfloat162_rn(low, high);
+      w[i] = *reinterpret_cast<const uint32_t*>(&b);
+    } else {
+      const __half2 b = __floats2half2_rn(low, high);
+      w[i] = *reinterpret_cast<const uint32_t*>(&b);
+    }
+  }
+  uint16_t* p = static_cast<uint16_t*>(row) + c;
+  if constexpr (P == 8) {
+    if (left >= 8) {
+      *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+      return;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    if (i < left) p[i] = static_cast<uint16_t>(w[i / 2] >> (16 * (i % 2)));
+  }
+}
+
+// Codes of P values.
+template <int P>
+__device__ __forceinline__ void store_codes(int8_t* row, int c, int left, const float (&v)[P], const RowCodes& codes) {
+  if constexpr (P == 8) {
+    const uint2 b = eight_codes(v, codes);
+    if (left >= 8) {
+      *reinterpret_cast<uint2*>(row + c) = b;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (i < left) row[c + i] = static_cast<int8_t>((i < 4 ? b.x : b.y) >> (8 * (i % 4)));
+      }
+    }
+  } else {
+    if (left > 0) row[c] = static_cast<int8_t>(one_code(v[0], codes));
+  }
+}
+
+// Over the row's threads; `shared` (one word for each warp) serves one reduction of a kernel.
+template <bool WARP>
+__device__ __forceinline__ uint32_t row_max(uint32_t v, uint32_t* shared) {
+  v = __reduce_max_sync(0xFFFFFFFFu, v);
+  if constexpr (WARP) return v;
+  const int lane = threadIdx.x & 31;
+  if (lane == 0) shared[threadIdx.x >> 5] = v;
+  __syncthreads();
+  return __reduce_max_sync(0xFFFFFFFFu, lane < static_cast<int>(blockDim.x >> 5) ? shared[lane] : 0u);
+}
+
+template <bool WARP>
+__device__ __forceinline__ double row_sum(double v, double* shared) {
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, d);
-  if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = v;
+  if constexpr (WARP) return v;
+  const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  if (lane == 0) shared[threadIdx.x >> 5] = v;
   __syncthreads();
-  double all = 0.0;
+  if (warps <= 12) {
+    v = shared[0];
+    for (int w = 1; w < warps; ++w) v += shared[w];
+    return v;
+  }
+  v = lane < warps ? shared[lane] : 0.0;
 #pragma unroll
-  for (int w = 0; w < THREADS / 32; ++w) all += shared[w];
-  __syncthreads();
-  return all;
+  for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, d);
+  return v;
 }
 
-constexpr int kRowThreads = 256;
+constexpr int kWarpRows = 8;  // rows of a CTA where each belongs to a warp
+
+template <bool WARP>
+__device__ __forceinline__ int row_of_thread() {
+  return WARP ? static_cast<int>(blockIdx.x) * kWarpRows + static_cast<int>(threadIdx.x >> 5)
+              : static_cast<int>(blockIdx.x);
+}
+
+struct QuantizeParams {
+  const void* x;
+  const int* source;  // or null
+  int8_t* q;
+  float* scales;
+  long long ldx, ldq;
+  int rows, tokens, k;
+  int x_kind;
+};
 
 // Row r of the codes = row source[r] (or r) of x. A source row outside [0, tokens) leaves the
 // row's codes and its scale as they were.
-template <typename In>
-__global__ void __launch_bounds__(kRowThreads)
-int8_quantize_kernel(const In* __restrict__ x, long long ldx, const int* __restrict__ source,
-                     int rows, int tokens, int k, int8_t* __restrict__ q, long long ldq,
-                     float* __restrict__ scales) {
-  __shared__ uint32_t shared[kRowThreads / 32];
-  for (int r = blockIdx.x; r < rows; r += gridDim.x) {
-    const int t = source != nullptr ? source[r] : r;
-    if (t < 0 || t >= tokens) continue;
-    const In* in = x + t * ldx;
-    uint32_t amax = 0;
-    for (int c = threadIdx.x; c < k; c += kRowThreads) {
-      amax = max(amax, magnitude_bits(to_float(in[c])));
+template <bool WIDE, int P, int N, int THREADS, bool WARP>
+__global__ void __launch_bounds__(THREADS) int8_quantize_kernel(const QuantizeParams p) {
+  __shared__ uint32_t maxima[32];
+  const int r = row_of_thread<WARP>();
+  if (r >= p.rows) return;
+  const int t = p.source != nullptr ? __ldg(p.source + r) : r;
+  if (t < 0 || t >= p.tokens) return;
+  const int step = P * (WARP ? 32 : P == 1 ? THREADS : blockDim.x);
+  const int first = P * (WARP ? threadIdx.x & 31 : threadIdx.x);
+  const void* in = static_cast<const uint8_t*>(p.x) + t * p.ldx * (WIDE ? 4 : 2);
+  Raw<WIDE, P> raw[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) raw[j] = load_raw<WIDE, P>(in, first + step * j, p.k - first - step * j);
+  // 16-bit magnitudes order like their bits, too: the largest of the negative ones is the largest
+  // unsigned pattern, that of the positive ones the largest signed one.
+  uint32_t amax = 0, positive = 0;
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    if constexpr (WIDE) {
+#pragma unroll
+      for (int i = 0; i < P; ++i) amax = max(amax, raw[j].w[i] & 0x7FFFFFFFu);
+    } else if constexpr (P == 8) {
+      amax = __vimax3_u16x2(__vimax3_u16x2(amax, raw[j].w[0], raw[j].w[1]), raw[j].w[2], raw[j].w[3]);
+      positive = __vimax3_s16x2(__vimax3_s16x2(positive, raw[j].w[0], raw[j].w[1]), raw[j].w[2], raw[j].w[3]);
+    } else {
+      amax = max(amax, raw[j].w[0] & 0x7FFFu);
     }
-    amax = block_max<kRowThreads>(amax, shared);
-    const float scale = row_scale(amax);
-    const bool live = row_has_codes(amax, scale);
-    for (int c = threadIdx.x; c < k; c += kRowThreads) {
-      q[r * ldq + c] = static_cast<int8_t>(live ? row_code(to_float(in[c]), scale) : 0);
-    }
-    if (threadIdx.x == 0) scales[r] = scale;
   }
+  const bool half = p.x_kind == 2;
+  if constexpr (!WIDE) {
+    if constexpr (P == 8) amax = __vmaxu2(amax & 0x7FFF7FFFu, positive);
+    const uint32_t both = max(amax & 0xFFFFu, amax >> 16);
+    amax = half ? magnitude_bits(__half2float(__ushort_as_half(static_cast<unsigned short>(both))))
+                : both << 16;
+  }
+  amax = row_max<WARP>(amax, maxima);
+  const RowCodes row = row_codes(amax);
+  int8_t* out = p.q + r * p.ldq;
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const int c = first + step * j;
+    if (c < p.k) {
+      float v[P];
+      unpack<WIDE, P>(raw[j], half, v);
+      store_codes<P>(out, c, p.k - c, v, row);
+    }
+  }
+  if (first == 0) p.scales[r] = row.scale;
 }
 
 // ---------------------------------------------------------------------------
@@ -127,9 +384,213 @@ struct NormParams {
   long long ldx, ldres, ldr, ldy;
   int tokens, hidden, tokens_per_gate;
   float residual_scale;
-  double eps;
+  double eps, inverse_hidden;
   int x_kind, residual_kind, y_kind;  // NVFP4_IN_*; y_kind -1: codes
 };
+
+__device__ __forceinline__ const void* row_at(const void* p, long long element, int kind) {
+  return static_cast<const uint8_t*>(p) + element * (kind == 0 ? 4 : 2);
+}
+
+__device__ __forceinline__ void* row_at(void* p, long long element, int kind) {
+  return static_cast<uint8_t*>(p) + element * (kind == 0 ? 4 : 2);
+}
+
+// 1 / sqrt(mean + eps) of a row, rounded to FP32 once. The sum is taken in 64 bits: its value
+// then does not depend, at FP32's precision, on how a row is split over threads, and codes that
+// lie next to a border come out the same for every split. Two steps of Newton's iteration for
+// m^(-1/2) in 64 bits, r += r (1 - m r^2) / 2, square the error of FP32's estimate twice (2^-21 to
+// below 2^-52); the 64-bit square root and quotient are left to means FP32 cannot hold.
+__device__ __forceinline__ float row_rstd(double sum, double inverse_hidden, double eps) {
+  const double m = fma(sum, inverse_hidden, eps);
+  if (!(m > 1e-30 && m < 1e30)) return static_cast<float>(1.0 / sqrt(m));
+  double r = rsqrtf(static_cast<float>(m));
+#pragma unroll
+  for (int i = 0; i < 2; ++i) r = fma(0.5 * r, fma(-m * r, r, 1.0), r);
+  return static_cast<float>(r);
+}
+
+// Sums of squares in four chains: a chain of 32 dependent 64-bit additions took longer than the
+// loads.
+struct SquareSum {
+  double s[4] = {0.0, 0.0, 0.0, 0.0};
+  template <int P>
+  __device__ __forceinline__ void add(const float (&v)[P], int piece) {
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      const double d = v[i];
+      double& chain = s[(piece * P + i) % 4];
+      chain = fma(d, d, chain);
+    }
+  }
+  __device__ __forceinline__ double total() const { return (s[0] + s[1]) + (s[2] + s[3]); }
+};
+
+// Two products or sums an instruction, each rounded on its own: a row's values, and with them its
+// codes, are those of the separate operations. (A packed sum behind a packed product was fused in
+// spite of its rounding mode: where one follows the other the product is taken unpacked.)
+__device__ __forceinline__ float2 product2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t"
+      ".reg .b64 x, y;\n\t"
+      "mov.b64 x, {%2, %3};\n\t"
+      "mov.b64 y, {%4, %5};\n\t"
+      "mul.rn.f32x2 x, x, y;\n\t"
+      "mov.b64 {%0, %1}, x;\n\t"
+      "}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+
+__device__ __forceinline__ float2 sum2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t"
+      ".reg .b64 x, y;\n\t"
+      "mov.b64 x, {%2, %3};\n\t"
+      "mov.b64 y, {%4, %5};\n\t"
+      "add.rn.f32x2 x, x, y;\n\t"
+      "mov.b64 {%0, %1}, x;\n\t"
+      "}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+
+template <int P>
+__device__ __forceinline__ void scale_by(float (&v)[P], float s) {
+#pragma unroll
+  for (int i = 0; i + 1 < P; i += 2) {
+    const float2 f = product2(make_float2(v[i], v[i + 1]), make_float2(s, s));
+    v[i] = f.x;
+    v[i + 1] = f.y;
+  }
+  if constexpr (P == 1) v[0] = __fmul_rn(v[0], s);
+}
+
+template <int P>
+__device__ __forceinline__ void multiply(float (&v)[P], const float (&w)[P]) {
+#pragma unroll
+  for (int i = 0; i + 1 < P; i += 2) {
+    const float2 f = product2(make_float2(v[i], v[i + 1]), make_float2(w[i], w[i + 1]));
+    v[i] = f.x;
+    v[i + 1] = f.y;
+  }
+  if constexpr (P == 1) v[0] = __fmul_rn(v[0], w[0]);
+}
+
+template <int P>
+__device__ __forceinline__ void add(float (&v)[P], const float (&w)[P]) {
+#pragma unroll
+  for (int i = 0; i + 1 < P; i += 2) {
+    const float2 f = sum2(make_float2(v[i], v[i + 1]), make_float2(w[i], w[i + 1]));
+    v[i] = f.x;
+    v[i + 1] = f.y;
+  }
+  if constexpr (P == 1) v[0] = __fadd_rn(v[0], w[0]);
+}
+
+template <bool X_WIDE, bool R_WIDE, int P, int N, int THREADS, bool WARP>
+__global__ void __launch_bounds__(THREADS) residual_norm_kernel(const NormParams p) {
+  __shared__ double post_sums[32], next_sums[32];
+  __shared__ uint32_t maxima[32];
+  const int t = row_of_thread<WARP>();
+  if (t >= p.tokens) return;
+  const int hidden = p.hidden;
+  const int step = P * (WARP ? 32 : P == 1 ? THREADS : blockDim.x);
+  const int first = P * (WARP ? threadIdx.x & 31 : threadIdx.x);
+  Raw<X_WIDE, P> raw_x[N];
+  Raw<R_WIDE, P> raw_r[N];
+  const void* x_row = row_at(p.x, t * p.ldx, p.x_kind);
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    raw_x[j] = load_raw<X_WIDE, P>(x_row, first + step * j, hidden - first - step * j);
+  }
+  if (p.residual != nullptr) {
+    const void* res_row = row_at(p.residual, t * p.ldres, p.residual_kind);
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      raw_r[j] = load_raw<R_WIDE, P>(res_row, first + step * j, hidden - first - step * j);
+    }
+  }
+  float v[N][P];
+#pragma unroll
+  for (int j = 0; j < N; ++j) unpack<X_WIDE, P>(raw_x[j], p.x_kind == 2, v[j]);
+  if (p.post_weight != nullptr) {
+    SquareSum sum;
+#pragma unroll
+    for (int j = 0; j < N; ++j) sum.add(v[j], j);
+    const float rstd = row_rstd(row_sum<WARP>(sum.total(), post_sums), p.inverse_hidden, p.eps);
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      float w[P];
+      load_weights<P>(p.post_weight, first + step * j, hidden - first - step * j, w);
+      scale_by(v[j], rstd);
+      multiply(v[j], w);
+    }
+  }
+  if (p.gate != nullptr) {
+    const float* gate = p.gate + static_cast<long long>(t / p.tokens_per_gate) * hidden;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      float g[P];
+      load_weights<P>(gate, first + step * j, hidden - first - step * j, g);
+      multiply(v[j], g);
+    }
+  }
+  if (p.residual != nullptr) {
+    void* r_row = row_at(p.r, t * p.ldr, p.residual_kind);
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int c = first + step * j;
+      float res[P];
+      unpack<R_WIDE, P>(raw_r[j], p.residual_kind == 2, res);
+#pragma unroll
+      for (int i = 0; i < P; ++i) res[i] = __fmul_rn(res[i], p.residual_scale);
+      add(v[j], res);
+      if (c < hidden) store_values<P>(r_row, c, hidden - c, p.residual_kind, v[j]);
+    }
+  }
+  if (p.next_weight == nullptr) return;
+  SquareSum sum;
+#pragma unroll
+  for (int j = 0; j < N; ++j) sum.add(v[j], j);
+  const float rstd = row_rstd(row_sum<WARP>(sum.total(), next_sums), p.inverse_hidden, p.eps);
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    float w[P];
+    load_weights<P>(p.next_weight, first + step * j, hidden - first - step * j, w);
+    scale_by(v[j], rstd);
+    multiply(v[j], w);
+  }
+  if (p.y_kind >= 0) {
+    void* y_row = row_at(p.y, t * p.ldy, p.y_kind);
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int c = first + step * j;
+      if (c < hidden) store_values<P>(y_row, c, hidden - c, p.y_kind, v[j]);
+    }
+    return;
+  }
+  uint32_t amax = 0;
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+#pragma unroll
+    for (int i = 0; i < P; ++i) amax = max(amax, magnitude_bits(v[j][i]));
+  }
+  const RowCodes row = row_codes(row_max<WARP>(amax, maxima));
+  int8_t* y_row = static_cast<int8_t*>(p.y) + t * p.ldy;
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const int c = first + step * j;
+    if (c < hidden) store_codes<P>(y_row, c, hidden - c, v[j], row);
+  }
+  if (first == 0) p.scales[t] = row.scale;
+}
+
+// ---------------------------------------------------------------------------
+// Rows too long for registers
+// ---------------------------------------------------------------------------
 
 __device__ __forceinline__ float load_kind(const void* p, long long i, int kind) {
   if (kind == 0) return static_cast<const float*>(p)[i];
@@ -137,78 +598,27 @@ __device__ __forceinline__ float load_kind(const void* p, long long i, int kind)
   return to_float(static_cast<const __half*>(p)[i]);
 }
 
-__device__ __forceinline__ void store_kind(void* p, long long i, int kind, float v) {
-  if (kind == 0) {
-    static_cast<float*>(p)[i] = v;
-  } else if (kind == 1) {
-    static_cast<__nv_bfloat16*>(p)[i] = from_float<__nv_bfloat16>(v);
-  } else {
-    static_cast<__half*>(p)[i] = from_float<__half>(v);
+// A CTA to a row, which is read twice (the second time mostly from the caches).
+__global__ void __launch_bounds__(1024) int8_quantize_long_kernel(const QuantizeParams p) {
+  __shared__ uint32_t maxima[32];
+  const int r = blockIdx.x;
+  const int t = p.source != nullptr ? __ldg(p.source + r) : r;
+  if (t < 0 || t >= p.tokens) return;
+  uint32_t amax = 0;
+#pragma unroll 8
+  for (int c = threadIdx.x; c < p.k; c += 1024) {
+    amax = max(amax, magnitude_bits(load_kind(p.x, t * p.ldx + c, p.x_kind)));
   }
-}
-
-// 1 / sqrt(mean + eps) of a row, rounded to FP32 once. The sum is taken in 64 bits: its value
-// then does not depend, at FP32's precision, on how a row is split over threads, and codes that
-// lie next to a border come out the same for every split.
-__device__ __forceinline__ float row_rstd(double sum, int hidden, double eps) {
-  return static_cast<float>(1.0 / sqrt(sum / hidden + eps));
-}
-
-__global__ void __launch_bounds__(kRowThreads) residual_norm_kernel(const NormParams p) {
-  extern __shared__ float row[];
-  __shared__ double sums[kRowThreads / 32];
-  __shared__ uint32_t maxima[kRowThreads / 32];
-  for (int t = blockIdx.x; t < p.tokens; t += gridDim.x) {
-    double sum = 0.0;
-    for (int c = threadIdx.x; c < p.hidden; c += kRowThreads) {
-      const float v = load_kind(p.x, t * p.ldx + c, p.x_kind);
-      row[c] = v;
-      sum += static_cast<double>(v) * v;
-    }
-    if (p.post_weight != nullptr) sum = block_sum<kRowThreads>(sum, sums);
-    const float post = p.post_weight != nullptr ? row_rstd(sum, p.hidden, p.eps) : 1.0f;
-    sum = 0.0;
-    for (int c = threadIdx.x; c < p.hidden; c += kRowThreads) {
-      float v = row[c];
-      if (p.post_weight != nullptr) v = __fmul_rn(__fmul_rn(v, post), p.post_weight[c]);
-      if (p.gate != nullptr) {
-        v = __fmul_rn(v, p.gate[static_cast<long long>(t / p.tokens_per_gate) * p.hidden + c]);
-      }
-      if (p.residual != nullptr) {
-        v = __fadd_rn(__fmul_rn(load_kind(p.residual, t * p.ldres + c, p.residual_kind),
-                                p.residual_scale), v);
-        store_kind(p.r, t * p.ldr + c, p.residual_kind, v);
-      }
-      row[c] = v;
-      sum += static_cast<double>(v) * v;
-    }
-    if (p.next_weight == nullptr) continue;
-    sum = block_sum<kRowThreads>(sum, sums);
-    const float next = row_rstd(sum, p.hidden, p.eps);
-    uint32_t amax = 0;
-    for (int c = threadIdx.x; c < p.hidden; c += kRowThreads) {
-      const float v = __fmul_rn(__fmul_rn(row[c], next), p.next_weight[c]);
-      if (p.y_kind >= 0) {
-        store_kind(p.y, t * p.ldy + c, p.y_kind, v);
-      } else {
-        row[c] = v;
-        amax = max(amax, magnitude_bits(v));
-      }
-    }
-    if (p.y_kind >= 0) continue;
-    amax = block_max<kRowThreads>(amax, maxima);
-    const float scale = row_scale(amax);
-    const bool live = row_has_codes(amax, scale);
-    for (int c = threadIdx.x; c < p.hidden; c += kRowThreads) {
-      static_cast<int8_t*>(p.y)[t * p.ldy + c] =
-          static_cast<int8_t>(live ? row_code(row[c], scale) : 0);
-    }
-    if (threadIdx.x == 0) p.scales[t] = scale;
+  const RowCodes row = row_codes(row_max<false>(amax, maxima));
+#pragma unroll 8
+  for (int c = threadIdx.x; c < p.k; c += 1024) {
+    p.q[r * p.ldq + c] = static_cast<int8_t>(one_code(load_kind(p.x, t * p.ldx + c, p.x_kind), row));
   }
+  if (threadIdx.x == 0) p.scales[r] = row.scale;
 }
 
 // ---------------------------------------------------------------------------
-// Products
+// Products and routing
 // ---------------------------------------------------------------------------
 
 // x * sigmoid(x).
