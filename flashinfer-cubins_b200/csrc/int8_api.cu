@@ -95,10 +95,9 @@ TileKernel tile_kernel(int ctas, bool gated) {
   return gated ? int8_tile_kernel<1, true> : int8_tile_kernel<1, false>;
 }
 
-// Static shared memory of the kernels (the same in all four, to within padding) and the slack that
-// aligns the stages to 1,024 bytes come off what a block can have.
-constexpr int kSharedLimit = 232448;
-constexpr int kStaticShared = 10 * 1024;
+// What a block can have of shared memory, less the kernels' static share (barriers and the epilogue's
+// scales, 2.4 KB) and the slack that aligns the stages to 1,024 bytes.
+constexpr int kSharedLimit = 232448 - 3 * 1024;
 
 int encode(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims,
            const cuuint64_t* strides, const cuuint32_t* box) {
@@ -161,13 +160,14 @@ int launch_product(const Product& q, void* stream) {
   p.tile_tokens = tile_tokens;
   p.split = split;
   const int stage_bytes = kInt8WeightBytes + tile_tokens / ctas * 128;
-  p.stages = std::min(kInt8MaxStages, (kSharedLimit - kStaticShared - 1024) / stage_bytes);
-  const size_t shared = static_cast<size_t>(p.stages) * stage_bytes + 1024;
+  const int tables = 8 * (q.experts + 1);
+  p.stages = std::min(kInt8MaxStages, (kSharedLimit - 1024 - tables) / stage_bytes);
+  const size_t shared = static_cast<size_t>(p.stages) * stage_bytes + 1024 + tables;
 
   const TileKernel kernel = tile_kernel(ctas, q.gated);
   CUDA_TRY(cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                 cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                kSharedLimit - kStaticShared));
+                                kSharedLimit));
   const int group = split > 1 ? split : ctas;
   // A split tile is a cluster's only one; otherwise a CTA (or pair) on every SM walks the tiles.
   const long long groups = split > 1 ? tiles : std::min<long long>(tiles, sms / ctas);

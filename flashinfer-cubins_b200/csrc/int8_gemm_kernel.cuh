@@ -8,9 +8,9 @@
 // channels of one token at a time, which are neighbours in D: every store instruction of a warp
 // is one run of 64 or 128 bytes, for any n, ldd and alignment, with no staging.
 //
-// Warps of a CTA (192 threads): 0 loads (one thread issues cp.async.bulk.tensor into a ring of
+// Warps of a CTA: 0 loads (one thread issues cp.async.bulk.tensor into a ring of
 // stages of 128 k), 1 issues tcgen05.mma.kind::i8 (32 k each) into one of two accumulators in
-// tensor memory, 2-5 take the other accumulator out, scale and store it. CTAS = 2: a pair of CTAs
+// tensor memory, the others take the other accumulator out, scale and store it. CTAS = 2: a pair of CTAs
 // on neighbouring SMs works on 256 channel rows with tcgen05.mma.cta_group::2; each loads its own
 // 128 rows of B and half of the tile's tokens.
 //
@@ -29,7 +29,9 @@
 
 namespace nvfp4 {
 
-constexpr int kInt8Threads = 192;
+constexpr int kInt8EpilogueWarps = 8;
+constexpr int kInt8Parts = kInt8EpilogueWarps / 4;  // warps that share a quarter of tensor memory's lanes
+constexpr int kInt8Threads = 64 + 32 * kInt8EpilogueWarps;
 constexpr int kInt8WeightBytes = 128 * 128;  // a stage's rows of B
 constexpr int kInt8MaxStages = 12;
 constexpr int kInt8MaxExperts = 1024;
@@ -185,9 +187,7 @@ int8_tile_kernel(const __grid_constant__ Int8TileParams p) {
   __shared__ alignas(8) uint64_t bar_empty[kInt8MaxStages];
   __shared__ alignas(8) uint64_t bar_acc_full[2];
   __shared__ alignas(8) uint64_t bar_acc_empty[2];
-  __shared__ alignas(16) float scale_stage[4][32];
-  __shared__ int tiles_before[kInt8MaxExperts + 1];  // token tiles of the experts before
-  __shared__ int first_row[kInt8MaxExperts + 1];
+  __shared__ alignas(16) float scale_stage[kInt8EpilogueWarps][32];
   __shared__ uint32_t tmem_base_slot;
   __shared__ int abort_flag;
 
@@ -199,6 +199,9 @@ int8_tile_kernel(const __grid_constant__ Int8TileParams p) {
   const int tile_tokens = p.tile_tokens;
   const int stages = p.stages;
   const uint32_t stage_bytes = kInt8WeightBytes + static_cast<uint32_t>(tile_tokens / CTAS) * 128u;
+  // Behind the stages: for every expert the token tiles of those before it, and its first row.
+  int* tiles_before = reinterpret_cast<int*>(dyn_smem + (smem_base - smem_u32(dyn_smem)) + stages * stage_bytes);
+  int* first_row = tiles_before + p.experts + 1;
   const uint32_t tmem_cols = p.split > 1 ? tile_tokens : 2 * tile_tokens;
 
   if (threadIdx.x == 0) {
@@ -208,7 +211,7 @@ int8_tile_kernel(const __grid_constant__ Int8TileParams p) {
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(smem_u32(&bar_acc_full[i]), 1);
-      mbar_init(smem_u32(&bar_acc_empty[i]), 4 * CTAS);
+      mbar_init(smem_u32(&bar_acc_empty[i]), kInt8EpilogueWarps * CTAS);
     }
     abort_flag = 0;
     mbar_fence_init();
@@ -413,7 +416,8 @@ int8_tile_kernel(const __grid_constant__ Int8TileParams p) {
   } else {
     // ------------------------------------------------------------------ epilogue
     const int quarter = warp & 3;
-    float* sa_stage = scale_stage[quarter];
+    const int part = (warp - 2) / 4;  // this warp's chunks of 32 tokens: part, part + kInt8Parts, ...
+    float* sa_stage = scale_stage[warp - 2];
     const uint32_t leader_acc_empty0 = CTAS == 1 ? smem_u32(&bar_acc_empty[0])
                                                  : cluster_map_shared(smem_u32(&bar_acc_empty[0]), 0);
     uint32_t acc = 0, acc_phase = 0;
@@ -437,7 +441,7 @@ int8_tile_kernel(const __grid_constant__ Int8TileParams p) {
       if (p.split > 1) {
         // Partial sums to shared memory (the stages are free: every MMA that read them is done),
         // [token][channel row]; after the cluster's barrier each CTA adds up its share of tokens.
-        for (int c = 0; c < tile.columns; c += 32) {
+        for (int c = 32 * part; c < tile.columns; c += 32 * kInt8Parts) {
           uint32_t r[32];
           tmem_load_32(taddr + c, r);
           tmem_load_wait();
@@ -452,7 +456,7 @@ int8_tile_kernel(const __grid_constant__ Int8TileParams p) {
         c_begin = tile.columns * static_cast<int>(rank) / p.split;
         c_end = tile.columns * (static_cast<int>(rank) + 1) / p.split;
       }
-      for (int c = c_begin; c < min(c_end, tile.tokens); c += 32) {
+      for (int c = c_begin + 32 * part; c < min(c_end, tile.tokens); c += 32 * kInt8Parts) {
         const int count = min(min(c_end, tile.tokens) - c, 32);
         sa_stage[lane] = lane < count ? __ldg(p.a_scales + tile.m0 + c + lane) : 0.0f;
         uint32_t r[32];
