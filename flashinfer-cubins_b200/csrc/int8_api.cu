@@ -4,6 +4,7 @@
 #include "../../include/nvfp4_b200.h"
 
 #include <algorithm>
+#include <cmath>
 #include <cstdint>
 #include <cstdio>
 
@@ -90,20 +91,23 @@ int check_product(const Product& p) {
 
 using TileKernel = void (*)(Int8TileParams);
 
-TileKernel tile_kernel(int ctas, bool gated) {
-  if (ctas == 2) return gated ? int8_tile_kernel<2, true> : int8_tile_kernel<2, false>;
-  return gated ? int8_tile_kernel<1, true> : int8_tile_kernel<1, false>;
+TileKernel tile_kernel(int ctas, int sub, bool gated) {
+  if (ctas == 1) {
+    return gated ? int8_tile_kernel<1, 2, true> : int8_tile_kernel<1, 2, false>;
+  }
+  if (sub == 1) return gated ? int8_tile_kernel<2, 1, true> : int8_tile_kernel<2, 1, false>;
+  return gated ? int8_tile_kernel<2, 2, true> : int8_tile_kernel<2, 2, false>;
 }
 
 // What a block can have of shared memory, less the kernels' static share (barriers and the epilogue's
-// scales, 2.4 KB) and the slack that aligns the stages to 1,024 bytes.
-constexpr int kSharedLimit = 232448 - 3 * 1024;
+// scales, 4.4 KB) and the slack that aligns the stages to 1,024 bytes.
+constexpr int kSharedLimit = 232448 - 5 * 1024;
 
 int encode(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims,
            const cuuint64_t* strides, const cuuint32_t* box) {
   EncodeTiled encoder = nullptr;
   if (int rc = host_encoder(&encoder)) return rc;
-  const cuuint32_t ones[4] = {1, 1, 1, 1};
+  const cuuint32_t ones[5] = {1, 1, 1, 1, 1};
   const CUresult res = encoder(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, rank, const_cast<void*>(base), dims,
                                strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
                                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -114,32 +118,104 @@ int encode(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims,
   return 0;
 }
 
+// How a product is cut: CTAs that share a tile's MMAs, tokens of a tile, pieces of 128 k in a stage,
+// and parts of k.
+struct Tiling {
+  int ctas, tile_tokens, sub, split;
+};
+
+// Microseconds of a tiling by the measured costs of its parts (1.9 GHz):
+//   a step of 128 k   the largest of its loads (140 GB/s an SM), its MMAs (2 columns a clock; 4 x 32 k)
+//                     and the loops that issue them (0.135 us; with one piece a stage 0.2 us)
+//   a tile            its steps, or, where those are shorter, its epilogue: 1 us for every 32 tokens
+//                     of a warp; the last epilogue stands alone
+//   a pair            0.5 us for its cluster; a split 1.2 us and 0.02 us a token for the exchange of
+//                     partial sums
+//   everything        not less than the operands' bytes at 6 TB/s; and a tenth of the loads at 12 TB/s,
+//                     which decides between tilings that are otherwise alike
+// What the choice is worth (device time, rows x n x k): 256 x 4096 x 7168 takes 13.4 us in pairs on 64
+// tokens and 21.9 on 256, where 32 of 148 SMs work; 200 x 5120 x 5120 11.7 on 96 and 18.0 on 256; 16 x
+// 7168 x 2048 6.3 us with all of k in one CTA and 8.0 split in two; 32 x 4096 x 8192 11.6 split in four
+// and 23 whole; 16 experts of 8192 rows, gated 1536 x 4096, 93 in pairs on 256 tokens and 270 on 32.
+double tiling_us(const Product& q, const Tiling& t, int sms, double* tiles) {
+  const int groups = std::min(q.experts, q.rows);
+  const int per_group = (q.rows + groups - 1) / groups;
+  const int m_tiles = (per_group + t.tile_tokens - 1) / t.tile_tokens;
+  const int columns = ((per_group + m_tiles - 1) / m_tiles + 31) / 32 * 32;
+  const int channels = (q.gated ? 64 : 128) * t.ctas;
+  *tiles = static_cast<double>(groups) * m_tiles * ((q.n + channels - 1) / channels);
+  const double loads = (128.0 + static_cast<double>(columns) / t.ctas) * 128.0 / 140e3;
+  const double mmas = columns * 2.0 / 1900.0;
+  const double step = std::max(std::max(loads, mmas), t.sub == 2 ? 0.135 : 0.2);
+  const int chunks = columns / 32;
+  const double epilogue = (chunks + int8_parts(t.tile_tokens) - 1) / int8_parts(t.tile_tokens);
+  const int k_tiles = (q.k + 127) / 128;
+  const double rounds = std::ceil(*tiles * t.split / (sms / t.ctas));
+  const double work = rounds * std::max((k_tiles + t.split - 1) / t.split * step, epilogue) + epilogue +
+                      (t.ctas == 2 ? 0.5 : 0.0) + (t.split > 1 ? 1.2 + 0.02 * columns : 0.0);
+  const double width = q.gated ? 2.0 * q.n : q.n;
+  const double bytes = groups * width * q.k + static_cast<double>(q.rows) * (q.k + 2.0 * q.n);
+  const double loaded = *tiles * k_tiles * (128.0 * t.ctas + columns) * 128.0;
+  return std::max(work, bytes / 6e6) + 0.1 * loaded / 12e6;
+}
+
+Tiling choose_tiling(const Product& q, int sms) {
+  const int groups = std::min(q.experts, q.rows);
+  const int per_group = (q.rows + groups - 1) / groups;
+  // Groups differ in size: a tile that holds twice the average reads few weights twice.
+  const int widest = std::min(256, (per_group + 31) / 32 * 32);
+  const int narrowest = q.experts > 1 ? std::min(256, (2 * per_group + 31) / 32 * 32) : 32;
+  Tiling best{};
+  double best_us = 0.0;
+  for (int ctas = per_group > 32 ? 2 : 1; ctas >= 1; --ctas) {
+    const int least = std::max(narrowest, 32 * ctas);
+    for (int tokens = std::max(widest, least); tokens >= least; tokens -= 32) {
+      for (int split = 1; split <= (ctas == 1 ? 8 : 1); split *= 2) {
+        const Tiling t{ctas, tokens, ctas == 1 || tokens <= 128 ? 2 : 1, split};
+        double tiles = 0.0;
+        const double us = tiling_us(q, t, sms, &tiles);
+        if (split > 1 && (tiles * split > sms || split * 2 > (q.k + 127) / 128)) break;
+        if (best.ctas == 0 || us < best_us * 0.98) {
+          best = t;
+          best_us = us;
+        }
+      }
+    }
+  }
+  return best;
+}
+
 int launch_product(const Product& q, void* stream) {
   if (int rc = check_product(q)) return rc;
   if (q.rows == 0) return 0;
   const int sms = host_sm_count();
-  const int k_tiles = (q.k + 127) / 128;
-  const int per_group = (q.rows + q.experts - 1) / q.experts;
-  int ctas = per_group > 128 ? 2 : 1;
-  int tile_tokens = ctas == 2 ? 256 : per_group <= 32 ? 32 : per_group <= 64 ? 64 : 128;
-  int split = 1;
+  Tiling tiling = choose_tiling(q, sms);
+  const int ctas = tiling.ctas, tile_tokens = tiling.tile_tokens, split = tiling.split;
   const int channels = (q.gated ? 64 : 128) * ctas;
   const long long n_tiles = (q.n + channels - 1) / channels;
   // No routing makes more token tiles than this.
-  const long long m_tiles = q.rows / tile_tokens + std::min(q.experts, q.rows);
-  long long tiles = (q.experts == 1 ? (q.rows + tile_tokens - 1) / tile_tokens : m_tiles) * n_tiles;
-  if (ctas == 1) {
-    while (split < 8 && tiles * split * 2 <= sms && split * 2 <= k_tiles) split *= 2;
-  }
+  const long long m_tiles = q.experts == 1 ? (q.rows + tile_tokens - 1) / tile_tokens
+                                           : q.rows / tile_tokens + std::min(q.experts, q.rows);
+  const long long tiles = m_tiles * n_tiles;
 
   Int8TileParams p{};
-  const cuuint64_t b_dims[4] = {static_cast<cuuint64_t>(q.k), static_cast<cuuint64_t>(q.n),
-                                q.gated ? 2u : 1u, static_cast<cuuint64_t>(q.experts)};
   const cuuint64_t half = static_cast<cuuint64_t>(q.n) * q.ldb;
-  const cuuint64_t b_strides[3] = {static_cast<cuuint64_t>(q.ldb), half,
-                                   q.experts > 1 ? static_cast<cuuint64_t>(q.expert_stride) : 2 * half};
-  const cuuint32_t b_box[4] = {128, q.gated ? 16u : 128u, q.gated ? 2u : 1u, 1};
-  if (int rc = encode(&p.map_b, q.b, 4, b_dims, b_strides, b_box)) return rc;
+  const cuuint64_t expert = q.experts > 1 ? static_cast<cuuint64_t>(q.expert_stride) : 2 * half;
+  p.whole = q.gated && q.n % 16 == 0;
+  if (p.whole) {
+    const cuuint64_t dims[5] = {static_cast<cuuint64_t>(q.k), 16, 2, static_cast<cuuint64_t>(q.n) / 16,
+                                static_cast<cuuint64_t>(q.experts)};
+    const cuuint64_t strides[4] = {static_cast<cuuint64_t>(q.ldb), half,
+                                   16 * static_cast<cuuint64_t>(q.ldb), expert};
+    const cuuint32_t box[5] = {128, 16, 2, 4, 1};
+    if (int rc = encode(&p.map_b, q.b, 5, dims, strides, box)) return rc;
+  } else {
+    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(q.k), static_cast<cuuint64_t>(q.n),
+                                q.gated ? 2u : 1u, static_cast<cuuint64_t>(q.experts)};
+    const cuuint64_t strides[3] = {static_cast<cuuint64_t>(q.ldb), half, expert};
+    const cuuint32_t box[4] = {128, q.gated ? 16u : 128u, q.gated ? 2u : 1u, 1};
+    if (int rc = encode(&p.map_b, q.b, 4, dims, strides, box)) return rc;
+  }
   const cuuint64_t a_dims[2] = {static_cast<cuuint64_t>(q.k), static_cast<cuuint64_t>(q.rows)};
   const cuuint64_t a_strides[1] = {static_cast<cuuint64_t>(q.lda)};
   const cuuint32_t a_box[2] = {128, static_cast<cuuint32_t>(tile_tokens / ctas)};
@@ -159,12 +235,14 @@ int launch_product(const Product& q, void* stream) {
   p.out_kind = q.out_kind;
   p.tile_tokens = tile_tokens;
   p.split = split;
-  const int stage_bytes = kInt8WeightBytes + tile_tokens / ctas * 128;
+  p.tmem_columns = 32;
+  while (p.tmem_columns < (split > 1 ? 1 : 2) * tile_tokens) p.tmem_columns *= 2;
+  const int stage_bytes = tiling.sub * 128 * (128 + tile_tokens / ctas);
   const int tables = 8 * (q.experts + 1);
   p.stages = std::min(kInt8MaxStages, (kSharedLimit - 1024 - tables) / stage_bytes);
   const size_t shared = static_cast<size_t>(p.stages) * stage_bytes + 1024 + tables;
 
-  const TileKernel kernel = tile_kernel(ctas, q.gated);
+  const TileKernel kernel = tile_kernel(ctas, tiling.sub, q.gated);
   CUDA_TRY(cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                 cudaFuncAttributeMaxDynamicSharedMemorySize,
                                 kSharedLimit));
@@ -180,7 +258,7 @@ int launch_product(const Product& q, void* stream) {
   attribute[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t config{};
   config.gridDim = dim3(static_cast<unsigned int>(groups * group));
-  config.blockDim = dim3(kInt8Threads);
+  config.blockDim = dim3(int8_threads(tile_tokens));
   config.dynamicSmemBytes = shared;
   config.stream = static_cast<cudaStream_t>(stream);
   config.attrs = attribute;

@@ -29,16 +29,23 @@
 
 namespace nvfp4 {
 
-constexpr int kInt8EpilogueWarps = 8;
-constexpr int kInt8Parts = kInt8EpilogueWarps / 4;  // warps that share a quarter of tensor memory's lanes
-constexpr int kInt8Threads = 64 + 32 * kInt8EpilogueWarps;
-constexpr int kInt8WeightBytes = 128 * 128;  // a stage's rows of B
+// Epilogue warps: four (one for each quarter of tensor memory's lanes) for every 32 tokens of a tile,
+// up to sixteen. A tile of 256 tokens then leaves in two rounds of 32 tokens a warp; with four warps
+// the epilogue took longer than the MMAs of 4096 k (gated 1000 x 14336 x 4096: 153 us, now 84), and
+// warps without work only poll.
+constexpr int kInt8MaxParts = 4;
+constexpr int int8_parts(int tile_tokens) {
+  return tile_tokens / 32 < kInt8MaxParts ? tile_tokens / 32 : kInt8MaxParts;
+}
+constexpr int int8_threads(int tile_tokens) { return 64 + 128 * int8_parts(tile_tokens); }
 constexpr int kInt8MaxStages = 12;
 constexpr int kInt8MaxExperts = 1024;
 constexpr int kInt8Band = 8;  // token tiles that are walked together, channel tile by channel tile
 
 struct Int8TileParams {
-  CUtensorMap map_b;       // [experts][2 if gated][n][k], box 128 (gated: 2 x 16) rows of 128 bytes
+  // Weights: [experts][1][n][k], box 128 rows of 128 bytes. Gated: [experts][n / 16][2][16][k], box
+  // 4 x 2 x 16 rows, or where n is no multiple of 16 [experts][2][n][k], box 2 x 16 rows.
+  CUtensorMap map_b;
   CUtensorMap map_a;       // [rows][k], box of a whole tile's tokens (a pair: of half of them)
   CUtensorMap map_a_part;  // the same with a box of 32 (a pair: 16) rows
   const float* a_scales;
@@ -49,9 +56,11 @@ struct Int8TileParams {
   long long ldd;
   int rows, n, k, experts;
   int out_kind;
-  int tile_tokens;  // 32, 64, 128 or 256
+  int tile_tokens;  // a multiple of 32, at most 256
+  int tmem_columns;
   int stages;
   int split;
+  int whole;  // gated: one copy brings a stage's weights
 };
 
 // Set to a role's code when it abandons a wait; read and cleared by nvfp4_int8_status.
@@ -133,6 +142,24 @@ __device__ __forceinline__ void tma_weights(uint32_t dst, const void* map, uint3
 }
 
 template <int CTAS>
+__device__ __forceinline__ void tma_gated_weights(uint32_t dst, const void* map, uint32_t bar, int k,
+                                                  int channel_group, int expert) {
+  if constexpr (CTAS == 1) {
+    asm volatile(
+        "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, "
+        "%4, %4, %5, %6}], [%2];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(k), "r"(0), "r"(channel_group), "r"(expert)
+        : "memory");
+  } else {
+    asm volatile(
+        "cp.async.bulk.tensor.5d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%3, %4, %4, %5, %6}], [%2];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(k), "r"(0), "r"(channel_group), "r"(expert)
+        : "memory");
+  }
+}
+
+template <int CTAS>
 __device__ __forceinline__ void int8_commit(uint32_t bar) {
   if constexpr (CTAS == 1) {
     tc_commit(bar);
@@ -178,16 +205,15 @@ __device__ __forceinline__ void store_columns(T* d, long long step, const float 
   }
 }
 
-template <int CTAS, bool GATED>
-__global__ void __launch_bounds__(kInt8Threads, 1)
+template <int CTAS, int SUB, bool GATED>
+__global__ void __launch_bounds__(64 + 128 * kInt8MaxParts, 1)
 int8_tile_kernel(const __grid_constant__ Int8TileParams p) {
-  constexpr int kChannels = GATED ? 64 : 128;  // output channels of a CTA
   extern __shared__ uint8_t dyn_smem[];
   __shared__ alignas(8) uint64_t bar_full[kInt8MaxStages];
   __shared__ alignas(8) uint64_t bar_empty[kInt8MaxStages];
   __shared__ alignas(8) uint64_t bar_acc_full[2];
   __shared__ alignas(8) uint64_t bar_acc_empty[2];
-  __shared__ alignas(16) float scale_stage[kInt8EpilogueWarps][32];
+  __shared__ alignas(16) float scale_stage[4 * kInt8MaxParts][64];
   __shared__ uint32_t tmem_base_slot;
   __shared__ int abort_flag;
 
@@ -198,11 +224,15 @@ int8_tile_kernel(const __grid_constant__ Int8TileParams p) {
   const bool leader = CTAS == 1 || rank == 0;
   const int tile_tokens = p.tile_tokens;
   const int stages = p.stages;
-  const uint32_t stage_bytes = kInt8WeightBytes + static_cast<uint32_t>(tile_tokens / CTAS) * 128u;
+  const int parts = (static_cast<int>(blockDim.x) - 64) / 128;  // warps that share a quarter
+  constexpr int channels = GATED ? 64 : 128;  // output channels of a CTA
+  constexpr uint32_t weight_bytes = 128u * 128u;  // of a piece of 128 k
+  const uint32_t token_bytes = static_cast<uint32_t>(tile_tokens / CTAS) * 128u;
+  const uint32_t stage_bytes = SUB * (weight_bytes + token_bytes);
   // Behind the stages: for every expert the token tiles of those before it, and its first row.
   int* tiles_before = reinterpret_cast<int*>(dyn_smem + (smem_base - smem_u32(dyn_smem)) + stages * stage_bytes);
   int* first_row = tiles_before + p.experts + 1;
-  const uint32_t tmem_cols = p.split > 1 ? tile_tokens : 2 * tile_tokens;
+  const uint32_t tmem_cols = p.tmem_columns;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < stages; ++s) {
@@ -211,7 +241,7 @@ int8_tile_kernel(const __grid_constant__ Int8TileParams p) {
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(smem_u32(&bar_acc_full[i]), 1);
-      mbar_init(smem_u32(&bar_acc_empty[i]), kInt8EpilogueWarps * CTAS);
+      mbar_init(smem_u32(&bar_acc_empty[i]), 4 * parts * CTAS);
     }
     abort_flag = 0;
     mbar_fence_init();
@@ -230,6 +260,11 @@ int8_tile_kernel(const __grid_constant__ Int8TileParams p) {
   grid_dependency_wait();
   grid_launch_dependents();
   if (warp == 0) {
+    if (lane == 0) {
+      prefetch_tensormap(&p.map_b);
+      prefetch_tensormap(&p.map_a);
+      prefetch_tensormap(&p.map_a_part);
+    }
     // First rows: the offsets cut to [0, rows], and where they decrease their running maximum, so
     // that no value of theirs makes groups overlap or reach outside. Then a prefix over the
     // experts' token tiles.
@@ -271,7 +306,7 @@ int8_tile_kernel(const __grid_constant__ Int8TileParams p) {
   volatile int* abort_ptr = &abort_flag;
 
   const int m_tiles = tiles_before[p.experts];
-  const int n_tiles = (p.n + kChannels * CTAS - 1) / (kChannels * CTAS);
+  const int n_tiles = (p.n + channels * CTAS - 1) / (channels * CTAS);
   const long long tiles = static_cast<long long>(m_tiles) * n_tiles;
   const int group = p.split > 1 ? p.split : CTAS;  // CTAs that share a tile
   const long long first_tile = blockIdx.x / group;
@@ -305,118 +340,142 @@ int8_tile_kernel(const __grid_constant__ Int8TileParams p) {
 
   if (warp == 0) {
     // ------------------------------------------------------------------ producer
+    // One thread runs the whole loop, here and in the MMA warp: electing it anew at every step cost
+    // 70 clocks of a step's 430.
     if (elect_one()) {
-      prefetch_tensormap(&p.map_b);
-      prefetch_tensormap(&p.map_a);
-      prefetch_tensormap(&p.map_a_part);
-    }
-    const uint32_t full0 = CTAS == 1 ? smem_u32(&bar_full[0])
-                                     : cluster_map_shared(smem_u32(&bar_full[0]), 0);
-    const uint32_t empty0 = smem_u32(&bar_empty[0]);
-    int stage = 0;
-    uint32_t phase = 0;
-    bool ok = true;
-    for (long long t = first_tile; ok && t < tiles; t += step) {
-      const Int8Tile tile = decode(t);
-      const int channel0 = (tile.n_tile * CTAS + static_cast<int>(CTAS == 2 ? rank : 0)) * kChannels;
-      const int share = tile.columns / CTAS;  // tokens this CTA loads
-      const int token0 = tile.m0 + static_cast<int>(CTAS == 2 ? rank : 0) * share;
-      const uint32_t bytes = kInt8WeightBytes + static_cast<uint32_t>(share) * 128u;
-      for (int kt = kt0; kt < kt1; ++kt) {
-        if (!mbar_wait(empty0 + 8 * stage, phase ^ 1u, abort_ptr)) {
-          int8_give_up(abort_ptr, kInt8ProducerTimeout);
-          ok = false;
-          break;
-        }
-        const uint32_t w_dst = smem_base + stage * stage_bytes;
-        const uint32_t t_dst = w_dst + kInt8WeightBytes;
-        const uint32_t bar = full0 + 8 * stage;
-        if (elect_one()) {
-          if (leader) mbar_expect_tx(smem_u32(&bar_full[stage]), CTAS * bytes);
-          if constexpr (GATED) {
+      const uint32_t full0 = CTAS == 1 ? smem_u32(&bar_full[0])
+                                       : cluster_map_shared(smem_u32(&bar_full[0]), 0);
+      const uint32_t empty0 = smem_u32(&bar_empty[0]);
+      int stage = 0;
+      uint32_t phase = 1;
+      uint32_t w_dst = smem_base;
+      bool ok = true;
+      for (long long t = first_tile; ok && t < tiles; t += step) {
+        const Int8Tile tile = decode(t);
+        const int channel0 = (tile.n_tile * CTAS + static_cast<int>(CTAS == 2 ? rank : 0)) * channels;
+        const int share = tile.columns / CTAS;  // tokens this CTA loads
+        const int token0 = tile.m0 + static_cast<int>(CTAS == 2 ? rank : 0) * share;
+        const uint32_t bytes = CTAS * (weight_bytes + static_cast<uint32_t>(share) * 128u);
+        int k = kt0 * 128;
+        for (int kt = kt0; kt < kt1; kt += SUB) {
+          if (!mbar_wait(empty0 + 8 * stage, phase, abort_ptr)) {
+            int8_give_up(abort_ptr, kInt8ProducerTimeout);
+            ok = false;
+            break;
+          }
+          const uint32_t bar = full0 + 8 * stage;
+          const uint32_t bar_here = smem_u32(&bar_full[stage]);
+          if (++stage == stages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+          const int parts = SUB == 1 ? 1 : min(SUB, kt1 - kt);
+          if (leader) mbar_expect_tx(bar_here, parts * bytes);
+          uint32_t w = w_dst, r = w_dst + SUB * weight_bytes;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              tma_weights<CTAS>(w_dst + 4096 * j, &p.map_b, bar, kt * 128, channel0 + 16 * j, tile.expert);
+          for (int i = 0; i < SUB; ++i) {
+            if (i >= parts) break;
+            if (GATED && p.whole) {
+              tma_gated_weights<CTAS>(w, &p.map_b, bar, k, channel0 / 16, tile.expert);
+            } else if constexpr (GATED) {
+#pragma unroll
+              for (int j = 0; j < channels; j += 16) {
+                tma_weights<CTAS>(w + 256 * j, &p.map_b, bar, k, channel0 + j, tile.expert);
+              }
+            } else {
+              tma_weights<CTAS>(w, &p.map_b, bar, k, channel0, tile.expert);
             }
-          } else {
-            tma_weights<CTAS>(w_dst, &p.map_b, bar, kt * 128, channel0, tile.expert);
-          }
-          if (tile.columns == tile_tokens) {
-            tma_rows<CTAS>(t_dst, &p.map_a, bar, kt * 128, token0);
-          } else {
-            for (int c = 0; c < share; c += 32 / CTAS) {
-              tma_rows<CTAS>(t_dst + c * 128, &p.map_a_part, bar, kt * 128, token0 + c);
+            if (tile.columns == tile_tokens) {
+              tma_rows<CTAS>(r, &p.map_a, bar, k, token0);
+            } else {
+              for (int c = 0; c < share; c += 32 / CTAS) {
+                tma_rows<CTAS>(r + c * 128, &p.map_a_part, bar, k, token0 + c);
+              }
             }
+            k += 128;
+            w += weight_bytes;
+            r += token_bytes;
           }
-        }
-        __syncwarp();
-        if (++stage == stages) {
-          stage = 0;
-          phase ^= 1u;
+          w_dst = stage == 0 ? smem_base : w_dst + stage_bytes;
         }
       }
     }
-    if (!ok || *abort_ptr != 0) {
+    __syncwarp();
+    if (*abort_ptr != 0) {
       // Copies may still be on their way into this CTA's memory: let them land.
       for (int i = 0; i < 64; ++i) __nanosleep(1000);
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issuer
-    if (leader) {
+    if (leader && elect_one()) {
       constexpr uint32_t kHi = (1024u >> 4) | (1u << 14) | (2u << 29);
       const uint32_t lo0 = ((smem_base >> 4) & 0x3FFFu) | (1u << 16);
       const uint32_t full0 = smem_u32(&bar_full[0]);
       const uint32_t empty0 = smem_u32(&bar_empty[0]);
       int stage = 0;
       uint32_t phase = 0;
-      uint32_t acc = 0, acc_phase = 0;
+      uint32_t acc = 0, acc_phase = 1;
+      uint32_t lo_w = lo0;
       bool ok = true;
       for (long long t = first_tile; ok && t < tiles; t += step) {
         const Int8Tile tile = decode(t);
         const uint32_t idesc = i8_instr_desc(128 * CTAS, static_cast<uint32_t>(tile.columns));
-        if (!mbar_wait(smem_u32(&bar_acc_empty[acc]), acc_phase ^ 1u, abort_ptr)) {
+        if (!mbar_wait(smem_u32(&bar_acc_empty[acc]), acc_phase, abort_ptr)) {
           int8_give_up(abort_ptr, kInt8MmaAccumTimeout);
           break;
         }
         tc_fence_after_sync();
         const uint32_t d = tmem_base + acc * tile_tokens;
         uint32_t accumulate = 0;
-        for (int kt = kt0; kt < kt1; ++kt) {
+        // k of this and the later stages. The last one's k beyond the depth is zero in both operands
+        // and not multiplied.
+        int left = min(p.k, kt1 * 128) - kt0 * 128;
+        for (int kt = kt0; kt < kt1; kt += SUB) {
           if (!mbar_wait(full0 + 8 * stage, phase, abort_ptr)) {
             int8_give_up(abort_ptr, kInt8MmaInputTimeout);
             ok = false;
             break;
           }
           tc_fence_after_sync();
-          const uint32_t lo_w = lo0 + ((stage * stage_bytes) >> 4);
-          const uint32_t lo_t = lo_w + (kInt8WeightBytes >> 4);
-          if (elect_one()) {
-            // The last stage's k beyond the depth is zero in both operands: not multiplied.
-            const int mmas = min(4, (p.k - kt * 128 + 31) / 32);
-            for (int j = 0; j < mmas; ++j) {
-              tc_mma_i8<CTAS>(d, pack_desc(lo_w + 2 * j, kHi), pack_desc(lo_t + 2 * j, kHi), idesc,
-                              j > 0 ? 1u : accumulate);
-            }
-            int8_commit<CTAS>(empty0 + 8 * stage);
-          }
-          __syncwarp();
-          accumulate = 1;
+          const uint32_t empty = empty0 + 8 * stage;
           if (++stage == stages) {
             stage = 0;
             phase ^= 1u;
           }
+          uint32_t w = lo_w, r = lo_w + SUB * (weight_bytes >> 4);
+#pragma unroll
+          for (int i = 0; i < SUB; ++i) {
+            if (left > 96) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                tc_mma_i8<CTAS>(d, pack_desc(w + 2 * j, kHi), pack_desc(r + 2 * j, kHi), idesc,
+                                j > 0 ? 1u : accumulate);
+              }
+            } else {
+              for (int j = 0; j * 32 < left; ++j) {
+                tc_mma_i8<CTAS>(d, pack_desc(w + 2 * j, kHi), pack_desc(r + 2 * j, kHi), idesc,
+                                j > 0 ? 1u : accumulate);
+              }
+            }
+            accumulate = 1;
+            left -= 128;
+            w += weight_bytes >> 4;
+            r += token_bytes >> 4;
+          }
+          int8_commit<CTAS>(empty);
+          lo_w = stage == 0 ? lo0 : lo_w + (stage_bytes >> 4);
         }
         if (!ok) break;
-        if (elect_one()) int8_commit<CTAS>(smem_u32(&bar_acc_full[acc]));
-        __syncwarp();
+        int8_commit<CTAS>(smem_u32(&bar_acc_full[acc]));
         acc ^= 1u;
         if (acc == 0) acc_phase ^= 1u;
       }
     }
+    __syncwarp();
   } else {
     // ------------------------------------------------------------------ epilogue
     const int quarter = warp & 3;
-    const int part = (warp - 2) / 4;  // this warp's chunks of 32 tokens: part, part + kInt8Parts, ...
+    const int part = (warp - 2) / 4;  // this warp's chunks of 32 tokens: part, part + parts, ...
     float* sa_stage = scale_stage[warp - 2];
     const uint32_t leader_acc_empty0 = CTAS == 1 ? smem_u32(&bar_acc_empty[0])
                                                  : cluster_map_shared(smem_u32(&bar_acc_empty[0]), 0);
@@ -424,24 +483,32 @@ int8_tile_kernel(const __grid_constant__ Int8TileParams p) {
     for (long long t = first_tile; t < tiles; t += step) {
       const Int8Tile tile = decode(t);
       // This lane's row of B: its channel in D, and its place among the scales.
-      const int channel0 = (tile.n_tile * CTAS + static_cast<int>(CTAS == 2 ? rank : 0)) * kChannels;
+      const int channel0 = (tile.n_tile * CTAS + static_cast<int>(CTAS == 2 ? rank : 0)) * channels;
       const int channel = GATED ? channel0 + quarter * 16 + (lane & 15) : channel0 + quarter * 32 + lane;
       const bool live = channel < p.n;
       const int width = GATED ? 2 * p.n : p.n;
       const int row = GATED && lane >= 16 ? p.n + channel : channel;
       const float sb = live ? __ldg(p.b_scales + static_cast<long long>(tile.expert) * width + row) : 0.0f;
       const float bias = live && p.bias != nullptr ? __ldg(p.bias + row) : 0.0f;
+      // Its tokens: all of the tile's, or with a split this CTA's share; their scales are fetched while
+      // the MMAs run.
+      const int c_begin = p.split > 1 ? tile.columns * static_cast<int>(rank) / p.split : 0;
+      const int c_end = min(p.split > 1 ? tile.columns * (static_cast<int>(rank) + 1) / p.split : tile.columns,
+                            tile.tokens);
+      for (int c = c_begin + 32 * part, i = 0; c < c_end; c += 32 * parts, i += 32) {
+        sa_stage[i + lane] = c + lane < c_end ? __ldg(p.a_scales + tile.m0 + c + lane) : 0.0f;
+      }
+      __syncwarp();
       if (!mbar_wait(smem_u32(&bar_acc_full[acc]), acc_phase, abort_ptr)) {
         int8_give_up(abort_ptr, kInt8EpilogueTimeout);
         break;
       }
       tc_fence_after_sync();
       const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + acc * tile_tokens;
-      int c_begin = 0, c_end = tile.columns;
       if (p.split > 1) {
         // Partial sums to shared memory (the stages are free: every MMA that read them is done),
         // [token][channel row]; after the cluster's barrier each CTA adds up its share of tokens.
-        for (int c = 32 * part; c < tile.columns; c += 32 * kInt8Parts) {
+        for (int c = 32 * part; c < tile.columns; c += 32 * parts) {
           uint32_t r[32];
           tmem_load_32(taddr + c, r);
           tmem_load_wait();
@@ -453,12 +520,10 @@ int8_tile_kernel(const __grid_constant__ Int8TileParams p) {
         }
         cluster_sync_all();
         partials_written = true;
-        c_begin = tile.columns * static_cast<int>(rank) / p.split;
-        c_end = tile.columns * (static_cast<int>(rank) + 1) / p.split;
       }
-      for (int c = c_begin + 32 * part; c < min(c_end, tile.tokens); c += 32 * kInt8Parts) {
-        const int count = min(min(c_end, tile.tokens) - c, 32);
-        sa_stage[lane] = lane < count ? __ldg(p.a_scales + tile.m0 + c + lane) : 0.0f;
+      const float* sa_next = sa_stage;
+      for (int c = c_begin + 32 * part; c < c_end; c += 32 * parts, sa_next += 32) {
+        const int count = min(c_end - c, 32);
         uint32_t r[32];
         if (p.split > 1) {
 #pragma unroll
@@ -475,22 +540,26 @@ int8_tile_kernel(const __grid_constant__ Int8TileParams p) {
           tmem_load_32(taddr + c, r);
           tmem_load_wait();
         }
-        __syncwarp();
         float v[32];
 #pragma unroll
         for (int i = 0; i < 32; i += 4) {
-          const float4 sa = *reinterpret_cast<const float4*>(sa_stage + i);
-          const float s[4] = {sa.x, sa.y, sa.z, sa.w};
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            v[i + j] = __fmul_rn(__fmul_rn(static_cast<float>(static_cast<int>(r[i + j])), s[j]), sb);
-          }
+          const float4 sa = *reinterpret_cast<const float4*>(sa_next + i);
+          const float2 sb2 = make_float2(sb, sb);
+          const float2 x = make_float2(static_cast<float>(static_cast<int>(r[i])),
+                                       static_cast<float>(static_cast<int>(r[i + 1])));
+          const float2 z = make_float2(static_cast<float>(static_cast<int>(r[i + 2])),
+                                       static_cast<float>(static_cast<int>(r[i + 3])));
+          const float2 low = product2(product2(x, make_float2(sa.x, sa.y)), sb2);
+          const float2 high = product2(product2(z, make_float2(sa.z, sa.w)), sb2);
+          v[i] = low.x;
+          v[i + 1] = low.y;
+          v[i + 2] = high.x;
+          v[i + 3] = high.y;
         }
         if (p.bias != nullptr) {
 #pragma unroll
           for (int i = 0; i < 32; ++i) v[i] = __fadd_rn(v[i], bias);
         }
-        __syncwarp();
         if constexpr (GATED) {
           // Of tokens 2i and 2i + 1 the gate lanes finish the first, the up lanes the second.
           float y[16];
@@ -524,7 +593,7 @@ int8_tile_kernel(const __grid_constant__ Int8TileParams p) {
         }
       }
       tc_fence_before_sync();
-      __syncwarp();
+      __syncwarp();  // also: every lane has read this tile's scales
       if (lane == 0) {
         if constexpr (CTAS == 1) {
           mbar_arrive(leader_acc_empty0 + 8 * acc);

@@ -30,6 +30,37 @@ __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) {
   return __float2bfloat16_rn(v);
 }
 
+// Two products or sums an instruction, each rounded on its own: a row's values, and with them its
+// codes, are those of the separate operations. (A packed sum behind a packed product was fused in
+// spite of its rounding mode: where one follows the other the product is taken unpacked.)
+__device__ __forceinline__ float2 product2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t"
+      ".reg .b64 x, y;\n\t"
+      "mov.b64 x, {%2, %3};\n\t"
+      "mov.b64 y, {%4, %5};\n\t"
+      "mul.rn.f32x2 x, x, y;\n\t"
+      "mov.b64 {%0, %1}, x;\n\t"
+      "}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+
+__device__ __forceinline__ float2 sum2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t"
+      ".reg .b64 x, y;\n\t"
+      "mov.b64 x, {%2, %3};\n\t"
+      "mov.b64 y, {%4, %5};\n\t"
+      "add.rn.f32x2 x, x, y;\n\t"
+      "mov.b64 {%0, %1}, x;\n\t"
+      "}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+
 // ---------------------------------------------------------------------------
 // Codes and scales of a row
 // ---------------------------------------------------------------------------
@@ -426,37 +457,6 @@ struct SquareSum {
   __device__ __forceinline__ double total() const { return (s[0] + s[1]) + (s[2] + s[3]); }
 };
 
-// Two products or sums an instruction, each rounded on its own: a row's values, and with them its
-// codes, are those of the separate operations. (A packed sum behind a packed product was fused in
-// spite of its rounding mode: where one follows the other the product is taken unpacked.)
-__device__ __forceinline__ float2 product2(float2 a, float2 b) {
-  float2 r;
-  asm("{\n\t"
-      ".reg .b64 x, y;\n\t"
-      "mov.b64 x, {%2, %3};\n\t"
-      "mov.b64 y, {%4, %5};\n\t"
-      "mul.rn.f32x2 x, x, y;\n\t"
-      "mov.b64 {%0, %1}, x;\n\t"
-      "}"
-      : "=f"(r.x), "=f"(r.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return r;
-}
-
-__device__ __forceinline__ float2 sum2(float2 a, float2 b) {
-  float2 r;
-  asm("{\n\t"
-      ".reg .b64 x, y;\n\t"
-      "mov.b64 x, {%2, %3};\n\t"
-      "mov.b64 y, {%4, %5};\n\t"
-      "add.rn.f32x2 x, x, y;\n\t"
-      "mov.b64 {%0, %1}, x;\n\t"
-      "}"
-      : "=f"(r.x), "=f"(r.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return r;
-}
-
 template <int P>
 __device__ __forceinline__ void scale_by(float (&v)[P], float s) {
 #pragma unroll
@@ -621,8 +621,14 @@ __global__ void __launch_bounds__(1024) int8_quantize_long_kernel(const Quantize
 // Products and routing
 // ---------------------------------------------------------------------------
 
-// x * sigmoid(x).
-__device__ __forceinline__ float silu(float x) { return x * __fdividef(1.0f, 1.0f + __expf(-x)); }
+// x * sigmoid(x) with the approximate exponential and reciprocal (2^-22 and 2^-23 relative): no slow
+// path where exp(-x) overflows, its reciprocal is 0 there.
+__device__ __forceinline__ float silu(float x) {
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x * -1.4426950408889634f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+  return x * r;
+}
 
 // Routing of pairs to unpadded groups: offsets[e] = number of pairs of the experts before e
 // (offsets[experts]: of all), and a cursor per expert that starts there.
