@@ -23,8 +23,6 @@ and contiguous. Weights are quantised by the same function, a scale for each out
 
 from __future__ import annotations
 
-import contextlib
-
 import torch
 
 from . import native
@@ -37,42 +35,54 @@ MAX_DEPTH = 131071  # k: sums of products of codes stay within 32 bits
 MAX_EXPERTS = 1024
 MAX_HIDDEN = 32768
 
+# Decode calls take a few microseconds on the GPU, so the host's share counts: devices are compared by
+# index, and the current stream's handle is read without making a Stream object (2 us less).
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
 _supported: dict[int, bool] = {}
 
 
-def _launch_on(device: torch.device):
-    """(context that makes ``device`` current, its current stream)."""
-    if device.type != "cuda":
-        raise RuntimeError(f"sm_100a code cannot run on {device}")
-    index = device.index
+def _check_device(index: int) -> None:
+    if index < 0:
+        raise RuntimeError("sm_100a code cannot run on the CPU")
     if index not in _supported:
         _supported[index] = native.device_supported(index)
     if not _supported[index]:
-        raise RuntimeError(f"sm_100a code cannot run on {device}")
-    stream = torch.cuda.current_stream(device).cuda_stream
+        raise RuntimeError(f"sm_100a code cannot run on cuda:{index}")
+
+
+def _launch(index: int, entry: str, *arguments) -> None:
+    """Call a C entry point on device ``index`` and its current stream."""
+    function = getattr(native.load(), entry)
     if index == torch.cuda.current_device():
-        return contextlib.nullcontext(), stream
-    return torch.cuda.device(device), stream
+        status = function(*arguments, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            status = function(*arguments, _raw_stream(index))
+    if status:
+        native.check(status)
 
 
 def _refuse_gradients(*tensors) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise ValueError("the INT8 operators have no backward; call them under torch.no_grad()")
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            raise ValueError("the INT8 operators have no backward; call them under torch.no_grad()")
 
 
 def _pitch(t: torch.Tensor, what: str) -> int:
     """Elements between the rows of ``t`` (its last but one dimension)."""
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
+    shape = t.shape
+    if shape[-1] > 1 and t.stride(-1) != 1:
         raise ValueError(f"{what}: elements of a row must be neighbours")
-    if t.shape[-2] > 1:
+    if shape[-2] > 1:
         return t.stride(-2)
-    return -(-t.shape[-1] // 16) * 16  # one row: nothing lies between
+    return -(-shape[-1] // 16) * 16  # one row: nothing lies between
 
 
-def _vector(t: torch.Tensor, shape: tuple, what: str, device: torch.device) -> int:
-    if t.dtype != torch.float32 or tuple(t.shape) != shape or not t.is_contiguous() or t.device != device:
-        raise ValueError(f"{what}: expected contiguous float32 {shape} on {device}, got {t.dtype} "
-                         f"{tuple(t.shape)} on {t.device}")
+def _vector(t: torch.Tensor, shape: tuple, what: str, index: int) -> int:
+    if t.dtype is not torch.float32 or t.shape != shape or not t.is_contiguous() or t.get_device() != index:
+        raise ValueError(f"{what}: expected contiguous float32 {shape} beside the first operand, got "
+                         f"{t.dtype} {tuple(t.shape)} on {t.device}")
     return t.data_ptr()
 
 
@@ -83,21 +93,19 @@ def empty_codes(rows: int, k: int, device: torch.device | str) -> torch.Tensor:
     return codes if pitch == k else codes[:, :k]
 
 
-def _codes(t: torch.Tensor, dims: int, what: str, device: torch.device) -> int:
-    if t.dtype != torch.int8 or t.dim() != dims or t.device != device:
-        raise ValueError(f"{what}: expected {dims}-d int8 on {device}, got {t.dtype} "
+def _codes(t: torch.Tensor, dims: int, what: str, index: int) -> int:
+    if t.dtype is not torch.int8 or t.dim() != dims or t.get_device() != index:
+        raise ValueError(f"{what}: expected {dims}-d int8 beside the first operand, got {t.dtype} "
                          f"{tuple(t.shape)} on {t.device}")
     return _pitch(t, what)
 
 
-def _output(out: torch.Tensor | None, rows: int, n: int, dtype: torch.dtype, device: torch.device):
-    """(tensor, elements between its rows)"""
-    if out is None:
-        return torch.empty((rows, n), dtype=dtype, device=device), n
-    if out.dtype != dtype or tuple(out.shape) != (rows, n) or out.device != device:
-        raise ValueError(f"out: expected {dtype} {(rows, n)} on {device}, got {out.dtype} "
+def _given(out: torch.Tensor, shape: tuple, dtype: torch.dtype, index: int, what: str) -> int:
+    """Elements between the rows of an output that the caller gave."""
+    if out.dtype is not dtype or out.shape != shape or out.get_device() != index:
+        raise ValueError(f"{what}: expected {dtype} {shape} beside the first operand, got {out.dtype} "
                          f"{tuple(out.shape)} on {out.device}")
-    return out, _pitch(out, "out")
+    return _pitch(out, what)
 
 
 def _width(width: int, gated: bool) -> int:
@@ -113,23 +121,26 @@ def gemm(a: torch.Tensor, b: torch.Tensor, a_scales: torch.Tensor, b_scales: tor
     ``b [n, k]``, summed exactly in 32-bit integers and rounded once to ``out_dtype`` (FP16, BF16 or
     FP32). With ``gated`` ``b`` is ``[2n, k]``, gate rows before up rows, and the result
     ``silu(gate) * up`` ``[m, n]``. ``out``: a tensor to write it to."""
-    device = a.device
-    _refuse_gradients(a_scales, b_scales, bias, out)
-    lda, ldb = _codes(a, 2, "a", device), _codes(b, 2, "b", device)
+    index = a.get_device()
+    if torch.is_grad_enabled():
+        _refuse_gradients(a_scales, b_scales, bias, out)
+    lda, ldb = _codes(a, 2, "a", index), _codes(b, 2, "b", index)
     (m, k), (width, depth) = a.shape, b.shape
     if depth != k:
         raise ValueError(f"a is {k} deep, b {depth}")
-    if out_dtype not in OUT_KINDS:
+    kind = OUT_KINDS.get(out_dtype)
+    if kind is None:
         raise ValueError(f"no output in {out_dtype}")
     n = _width(width, gated)
-    pa, pb = _vector(a_scales, (m,), "a_scales", device), _vector(b_scales, (width,), "b_scales", device)
-    pbias = None if bias is None else _vector(bias, (width,), "bias", device)
-    current, stream = _launch_on(device)
-    out, ldd = _output(out, m, n, out_dtype, device)
-    with current:
-        native.check(native.load().nvfp4_int8_gemm(
-            a.data_ptr(), lda, b.data_ptr(), ldb, pa, pb, pbias, out.data_ptr(), ldd, m, n, k,
-            OUT_KINDS[out_dtype], gated, stream))
+    pa, pb = _vector(a_scales, (m,), "a_scales", index), _vector(b_scales, (width,), "b_scales", index)
+    pbias = None if bias is None else _vector(bias, (width,), "bias", index)
+    _check_device(index)
+    if out is None:
+        out, ldd = torch.empty((m, n), dtype=out_dtype, device=a.device), n
+    else:
+        ldd = _given(out, (m, n), out_dtype, index, "out")
+    _launch(index, "nvfp4_int8_gemm", a.data_ptr(), lda, b.data_ptr(), ldb, pa, pb, pbias,
+            out.data_ptr(), ldd, m, n, k, kind, gated)
     return out
 
 
@@ -142,28 +153,31 @@ def grouped_gemm(a: torch.Tensor, b: torch.Tensor, a_scales: torch.Tensor, b_sca
     int32 tensor ``[experts + 1]`` on the device that does not decrease; it is read by the kernel,
     never by the host. Rows that no expert owns are left as they were in ``out`` (and hold anything
     in a result made here)."""
-    device = a.device
-    _refuse_gradients(a_scales, b_scales, out)
-    lda, ldb = _codes(a, 2, "a", device), _codes(b, 3, "b", device)
+    index = a.get_device()
+    if torch.is_grad_enabled():
+        _refuse_gradients(a_scales, b_scales, out)
+    lda, ldb = _codes(a, 2, "a", index), _codes(b, 3, "b", index)
     (rows, k), (experts, width, depth) = a.shape, b.shape
     if depth != k:
         raise ValueError(f"a is {k} deep, b {depth}")
-    if out_dtype not in OUT_KINDS:
+    kind = OUT_KINDS.get(out_dtype)
+    if kind is None:
         raise ValueError(f"no output in {out_dtype}")
     n = _width(width, gated)
-    pa = _vector(a_scales, (rows,), "a_scales", device)
-    pb = _vector(b_scales, (experts, width), "b_scales", device)
-    if (offsets.dtype != torch.int32 or tuple(offsets.shape) != (experts + 1,)
-            or not offsets.is_contiguous() or offsets.device != device):
-        raise ValueError(f"offsets: expected contiguous int32 {(experts + 1,)} on {device}, got "
-                         f"{offsets.dtype} {tuple(offsets.shape)} on {offsets.device}")
-    current, stream = _launch_on(device)
-    out, ldd = _output(out, rows, n, out_dtype, device)
-    with current:
-        native.check(native.load().nvfp4_int8_group_gemm(
-            a.data_ptr(), lda, b.data_ptr(), ldb, b.stride(0) if experts > 1 else 0, pa, pb,
-            offsets.data_ptr(), out.data_ptr(), ldd, experts, rows, n, k, OUT_KINDS[out_dtype],
-            gated, stream))
+    pa = _vector(a_scales, (rows,), "a_scales", index)
+    pb = _vector(b_scales, (experts, width), "b_scales", index)
+    if (offsets.dtype is not torch.int32 or offsets.shape != (experts + 1,)
+            or not offsets.is_contiguous() or offsets.get_device() != index):
+        raise ValueError(f"offsets: expected contiguous int32 {(experts + 1,)} beside the first operand, "
+                         f"got {offsets.dtype} {tuple(offsets.shape)} on {offsets.device}")
+    _check_device(index)
+    if out is None:
+        out, ldd = torch.empty((rows, n), dtype=out_dtype, device=a.device), n
+    else:
+        ldd = _given(out, (rows, n), out_dtype, index, "out")
+    _launch(index, "nvfp4_int8_group_gemm", a.data_ptr(), lda, b.data_ptr(), ldb,
+            b.stride(0) if experts > 1 else 0, pa, pb, offsets.data_ptr(), out.data_ptr(), ldd, experts,
+            rows, n, k, kind, gated)
     return out
 
 
@@ -175,32 +189,33 @@ def quantize_tokens(x: torch.Tensor, *, rows: torch.Tensor | None = None,
     0; a row with an infinity or a NaN has that as its scale and zero codes. ``rows`` (int32
     ``[R]`` on the device) gathers: row r of the codes is row ``rows[r]`` of ``x``; an index outside
     ``[0, tokens)`` leaves row r as it was. ``out``: codes and scales to write to."""
-    device = x.device
-    _refuse_gradients(x)
-    if x.dim() != 2 or x.dtype not in IN_KINDS:
+    index = x.get_device()
+    if torch.is_grad_enabled():
+        _refuse_gradients(x)
+    kind = IN_KINDS.get(x.dtype)
+    if x.dim() != 2 or kind is None:
         raise ValueError(f"x: expected 2-d FP32, BF16 or FP16, got {x.dtype} {tuple(x.shape)}")
     ldx = _pitch(x, "x")
     tokens, k = x.shape
     count, source = tokens, None
     if rows is not None:
-        if rows.dtype != torch.int32 or rows.dim() != 1 or not rows.is_contiguous() or rows.device != device:
-            raise ValueError(f"rows: expected contiguous 1-d int32 on {device}, got {rows.dtype} "
+        if rows.dtype is not torch.int32 or rows.dim() != 1 or not rows.is_contiguous() or rows.get_device() != index:
+            raise ValueError(f"rows: expected contiguous 1-d int32 beside the first operand, got {rows.dtype} "
                              f"{tuple(rows.shape)} on {rows.device}")
         count, source = rows.numel(), rows.data_ptr()
-    current, stream = _launch_on(device)
+    _check_device(index)
     if out is None:
+        device = x.device
+        ldq = -(-k // 16) * 16
         q = empty_codes(count, k, device)
         scales = torch.empty((count,), dtype=torch.float32, device=device)
+        ps = scales.data_ptr()
     else:
         q, scales = out
-        if tuple(q.shape) != (count, k):
-            raise ValueError(f"out: expected codes {(count, k)}, got {tuple(q.shape)}")
-    ldq = _codes(q, 2, "out", device)
-    ps = _vector(scales, (count,), "out", device)
-    with current:
-        native.check(native.load().nvfp4_int8_quantize(
-            x.data_ptr(), IN_KINDS[x.dtype], ldx, source, count, tokens, k, q.data_ptr(), ldq, ps,
-            stream))
+        ldq = _given(q, (count, k), torch.int8, index, "out")
+        ps = _vector(scales, (count,), "out", index)
+    _launch(index, "nvfp4_int8_quantize", x.data_ptr(), kind, ldx, source, count, tokens, k, q.data_ptr(),
+            ldq, ps)
     return q, scales
 
 
@@ -222,50 +237,56 @@ def residual_norm(x: torch.Tensor, residual: torch.Tensor | None = None, *,
     ``scales``; what is not made is None. ``gate`` is ``[hidden]`` or ``[gates, hidden]``, each row
     for ``tokens / gates`` consecutive tokens. Weights and gate are FP32. Without a residual only
     ``y = x / rms(x) * next_weight`` is made. ``residual_out`` may be ``residual`` itself."""
-    device = x.device
-    _refuse_gradients(x, residual, post_weight, gate, next_weight)
-    if x.dim() != 2 or x.dtype not in IN_KINDS:
+    index, device = x.get_device(), x.device
+    if torch.is_grad_enabled():
+        _refuse_gradients(x, residual, post_weight, gate, next_weight)
+    x_kind = IN_KINDS.get(x.dtype)
+    if x.dim() != 2 or x_kind is None:
         raise ValueError(f"x: expected 2-d FP32, BF16 or FP16, got {x.dtype} {tuple(x.shape)}")
-    tokens, hidden = x.shape
+    shape = x.shape
+    tokens, hidden = shape
     ldx = _pitch(x, "x")
     kind, pres, ldres = native.IN_F32, None, 0
     if residual is not None:
-        if residual.dtype not in IN_KINDS or residual.shape != x.shape or residual.device != device:
-            raise ValueError(f"residual: expected {tuple(x.shape)} on {device}, got "
+        kind = IN_KINDS.get(residual.dtype)
+        if kind is None or residual.shape != shape or residual.get_device() != index:
+            raise ValueError(f"residual: expected {tuple(shape)} beside the first operand, got "
                              f"{residual.dtype} {tuple(residual.shape)} on {residual.device}")
-        kind, pres, ldres = IN_KINDS[residual.dtype], residual.data_ptr(), _pitch(residual, "residual")
+        pres, ldres = residual.data_ptr(), _pitch(residual, "residual")
     elif residual_out is not None:
         raise ValueError("residual_out without a residual")
     if next_weight is None and (residual is None or quantize or out_dtype is not None):
         raise ValueError("next_weight is missing: there is nothing to norm, quantise or return")
     if quantize and out_dtype is not None:
         raise ValueError("codes have no out_dtype")
-    ppost = None if post_weight is None else _vector(post_weight, (hidden,), "post_weight", device)
-    pnext = None if next_weight is None else _vector(next_weight, (hidden,), "next_weight", device)
+    row = (hidden,)
+    ppost = None if post_weight is None else _vector(post_weight, row, "post_weight", index)
+    pnext = None if next_weight is None else _vector(next_weight, row, "next_weight", index)
     pgate, gates = None, 0
     if gate is not None:
         gates = gate.shape[0] if gate.dim() == 2 else 1
-        pgate = _vector(gate, (gates, hidden) if gate.dim() == 2 else (hidden,), "gate", device)
-    current, stream = _launch_on(device)
+        pgate = _vector(gate, (gates, hidden) if gate.dim() == 2 else row, "gate", index)
+    _check_device(index)
     r, pr, ldr = None, None, 0
     if residual is not None:
-        r, ldr = _output(residual_out, tokens, hidden, residual.dtype, device)
+        if residual_out is None:
+            r, ldr = torch.empty(shape, dtype=residual.dtype, device=device), hidden
+        else:
+            r, ldr = residual_out, _given(residual_out, shape, residual.dtype, index, "residual_out")
         pr = r.data_ptr()
     y, py, ldy, y_kind, scales, pscales = None, None, 0, native.NORM_CODES, None, None
     if next_weight is not None:
         if quantize:
-            y = empty_codes(tokens, hidden, device)
-            ldy = -(-hidden // 16) * 16
+            y, ldy = empty_codes(tokens, hidden, device), -(-hidden // 16) * 16
             scales = torch.empty((tokens,), dtype=torch.float32, device=device)
             pscales = scales.data_ptr()
         else:
             dtype = out_dtype or (x if residual is None else residual).dtype
-            if dtype not in IN_KINDS:
+            y_kind = IN_KINDS.get(dtype)
+            if y_kind is None:
                 raise ValueError(f"no output in {dtype}")
-            y, ldy, y_kind = torch.empty((tokens, hidden), dtype=dtype, device=device), hidden, IN_KINDS[dtype]
+            y, ldy = torch.empty(shape, dtype=dtype, device=device), hidden
         py = y.data_ptr()
-    with current:
-        native.check(native.load().nvfp4_residual_norm(
-            x.data_ptr(), IN_KINDS[x.dtype], ldx, pres, kind, ldres, ppost, pgate, gates,
-            residual_scale, pnext, eps, pr, ldr, py, y_kind, ldy, pscales, tokens, hidden, stream))
+    _launch(index, "nvfp4_residual_norm", x.data_ptr(), x_kind, ldx, pres, kind, ldres, ppost, pgate, gates,
+            residual_scale, pnext, eps, pr, ldr, py, y_kind, ldy, pscales, tokens, hidden)
     return r, y, scales

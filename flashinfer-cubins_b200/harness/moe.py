@@ -27,6 +27,9 @@ Layout choices that keep every stage a plain kernel launch on whole buffers:
   row counts and binds them once: a forward with a routing pattern seen before is one
   quantiser launch and two grouped GEMM launches, with nothing allocated, encoded or bound.
   It reads the row counts back (the plans' shapes are the host's).
+* ``Int8MoELayer`` is the layer on INT8 weights (``harness.int8``): the same stages on unpadded
+  rows, nothing read back, nothing kept between calls. ``MoEBlock`` puts the norms, the gate and
+  the residual scale of a transformer block around any of the layers.
 * ``RoutedMoELayer`` reads nothing back: its two plans take the experts' row counts from the
   device (``nvfp4_moe_plan_create`` and friends), all experts share buffers sized for the
   worst case, and one plan pair serves every routing, so a forward is a fixed sequence of
@@ -46,7 +49,7 @@ from collections.abc import Callable
 
 import torch
 
-from . import native
+from . import int8, native
 from .workloads import quantization as q
 
 ROW_BLOCK = 128
@@ -511,6 +514,114 @@ class RoutedMoELayer:
             return torch.empty((0, self.hidden), dtype=torch.float16, device=self.device)
         self._experts(rows, expert_ids.reshape(-1, 1))
         return self.y.index_select(0, self.row_of_pair[:rows.shape[0]])
+
+
+class Int8MoELayer:
+    """The layer on INT8 weights with a scale for each output channel: ``w13`` ``[E, 2I, H]`` (gate
+    rows then up rows) with FP32 ``w13_scales`` ``[E, 2I]``, ``w2`` ``[E, H, I]`` with ``w2_scales``
+    ``[E, H]``; ``quantize_int8_weights`` makes them. Every token is quantised with a scale of its
+    own into the rows of its experts, the gate is applied in the first product's epilogue, and its
+    BF16 result is quantised again for the second.
+
+    The experts' rows follow one another without padding and their offsets stay on the device
+    (``nvfp4_moe_offsets``), so a forward is a fixed sequence of nine launches that reads nothing
+    back. Its buffers belong to the forward: calls on several streams and captured graphs share
+    nothing but the weights. H is a multiple of 16 (of 8 for the combine), I of 16."""
+
+    def __init__(self, w13, w13_scales, w2, w2_scales):
+        if any(t.dim() != d for t, d in ((w13, 3), (w13_scales, 2), (w2, 3), (w2_scales, 2))):
+            raise ValueError("weights are [E, 2I, H] and [E, H, I], scales [E, 2I] and [E, H]")
+        experts, two_i, hidden = w13.shape
+        self.experts, self.hidden, self.inter = experts, hidden, two_i // 2
+        if two_i % 2 or tuple(w2.shape) != (experts, hidden, self.inter):
+            raise ValueError("w2 does not match w13")
+        if hidden % 16 or self.inter % 16:
+            raise ValueError("hidden and intermediate sizes must be multiples of 16")
+        if tuple(w13_scales.shape) != (experts, two_i) or tuple(w2_scales.shape) != (experts, hidden):
+            raise ValueError("scales do not match the weights")
+        if experts > 512:
+            raise ValueError("at most 512 experts")
+        self.device = w13.device
+        if self.device.type != "cuda" or not native.device_supported(self.device.index or 0):
+            raise RuntimeError(f"sm_100a code cannot run on {self.device}")
+        self.w13, self.w13_scales, self.w2, self.w2_scales = w13, w13_scales, w2, w2_scales
+
+    def forward(self, x: torch.Tensor, topk_ids: torch.Tensor, topk_weights: torch.Tensor) -> torch.Tensor:
+        """As ``MoELayer.forward`` (``x`` ``[T, H]`` FP32, BF16 or FP16, ids int32/int64 ``[T, K]``,
+        weights ``[T, K]``; FP32 ``[T, H]`` out). An id outside ``[0, E)`` adds nothing."""
+        tokens, choices = topk_ids.shape
+        if x.shape != (tokens, self.hidden) or topk_weights.shape != topk_ids.shape:
+            raise ValueError("activations, ids and weights do not match")
+        if any(t.device != self.device for t in (x, topk_ids, topk_weights)):
+            raise ValueError("operands must be on the layer's device")
+        pairs = tokens * choices
+        out = torch.empty((tokens, self.hidden), dtype=torch.float32, device=self.device)
+        if pairs == 0:
+            return out.zero_()
+        ids = topk_ids if topk_ids.dtype in (torch.int32, torch.int64) else topk_ids.long()
+        ids = ids.contiguous()
+        wide = ids.dtype == torch.int64
+        weights = topk_weights.float().contiguous()
+        word = dict(dtype=torch.int32, device=self.device)
+        with torch.cuda.device(self.device):
+            stream = torch.cuda.current_stream(self.device).cuda_stream
+            counts, cursors = torch.empty((2, self.experts), **word)
+            offsets = torch.empty((self.experts + 1,), **word)
+            row_of_pair, token_of_row = torch.empty((2, pairs), **word)
+            native.moe_count(ids.data_ptr(), wide, pairs, self.experts, counts.data_ptr(), stream)
+            native.moe_offsets(counts.data_ptr(), self.experts, offsets.data_ptr(), stream)
+            native.moe_place_offsets(ids.data_ptr(), wide, pairs, choices, self.experts,
+                                     offsets.data_ptr(), pairs, cursors.data_ptr(),
+                                     row_of_pair.data_ptr(), token_of_row.data_ptr(), stream)
+            a, a_scales = int8.quantize_tokens(x, rows=token_of_row)
+            h = int8.grouped_gemm(a, self.w13, a_scales, self.w13_scales, offsets, gated=True)
+            a, a_scales = int8.quantize_tokens(h)
+            y = int8.grouped_gemm(a, self.w2, a_scales, self.w2_scales, offsets,
+                                  out_dtype=torch.float16)
+            native.moe_combine(y.data_ptr(), row_of_pair.data_ptr(), weights.data_ptr(),
+                               out.data_ptr(), tokens, choices, self.hidden, stream)
+        return out
+
+
+def quantize_int8_weights(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Weights ``[E, N, K]`` -> INT8 codes and an FP32 scale for each output channel ``[E, N]``, as
+    ``Int8MoELayer`` and ``int8.grouped_gemm`` take them."""
+    experts, rows, k = w.shape
+    codes, scales = int8.quantize_tokens(w.reshape(experts * rows, k))
+    return codes.unflatten(0, (experts, rows)), scales.view(experts, rows)
+
+
+class MoEBlock:
+    """The norms around a mixture-of-experts layer (``MoELayer``, ``RoutedMoELayer`` or
+    ``Int8MoELayer``), fused with its gate and residual scale (``int8.residual_norm``)::
+
+        n = norm(residual) * pre_weight
+        residual = residual_scale * residual + gate * norm(layer(n)) * post_weight
+
+    One launch closes this block and opens the next. ``post_weight`` None: no norm behind the layer;
+    ``gate`` ``[H]`` or ``[gates, H]`` (each row for ``T / gates`` tokens) or None."""
+
+    def __init__(self, layer, pre_weight, post_weight=None, gate=None, residual_scale: float = 1.0,
+                 eps: float = 1e-6):
+        self.layer, self.pre_weight, self.post_weight = layer, pre_weight, post_weight
+        self.gate, self.residual_scale, self.eps = gate, residual_scale, eps
+
+    def enter(self, residual: torch.Tensor) -> torch.Tensor:
+        """``norm(residual) * pre_weight`` in the residual's type: what the router and the layer
+        see, where no block before this one has made it."""
+        return int8.residual_norm(residual, next_weight=self.pre_weight, eps=self.eps)[1]
+
+    def forward(self, residual: torch.Tensor, route: Callable, normed: torch.Tensor | None = None,
+                next_weight: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor | None]:
+        """``(new residual, norm(new residual) * next_weight)``: the second is the next block's
+        ``normed`` (None without ``next_weight``, the next block's ``pre_weight``). ``route(n)``
+        gives the expert ids and weights ``[T, K]`` of the normed tokens."""
+        if normed is None:
+            normed = self.enter(residual)
+        out = self.layer.forward(normed, *route(normed))
+        return int8.residual_norm(out, residual, post_weight=self.post_weight, gate=self.gate,
+                                  residual_scale=self.residual_scale, next_weight=next_weight,
+                                  eps=self.eps)[:2]
 
 
 def moe_forward(x, topk_ids, topk_weights, w13, w13_scales, w2, w2_scales,

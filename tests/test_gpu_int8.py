@@ -508,3 +508,135 @@ def test_offsets_and_placement_of_pairs():
     assert rows[7] == 2 and rows[3] == rows[4] == -1
     tokens = token_of_row.tolist()
     assert all(tokens[rows[i]] == i // 2 for i in (0, 1, 2, 5, 6, 7)) and tokens[6:] == [-1, -1]
+
+
+def moe_plain(x, ids, weights, w13, s13, w2, s2):
+    """The layer in 64 bits, with the two quantisers where the layer has them: the first on the
+    tokens (numpy's, bit for bit), the second on the gate rounded to BF16."""
+    experts, inter = w13.shape[0], w13.shape[1] // 2
+    q, s = np_quantized(x)
+    a = torch.from_numpy(q).to(DEV).double() * torch.from_numpy(s).to(DEV).double()[:, None]
+    out = torch.zeros(x.shape, dtype=torch.float64, device=DEV)
+    for e in range(experts):
+        token, choice = torch.nonzero(ids == e, as_tuple=True)
+        if token.numel() == 0:
+            continue
+        h = a[token] @ (w13[e].double() * s13[e].double()[:, None]).T
+        h = (h[:, :inter] * torch.sigmoid(h[:, :inter]) * h[:, inter:]).to(torch.bfloat16)
+        q2, t2 = np_quantized(h)
+        b = torch.from_numpy(q2).to(DEV).double() * torch.from_numpy(t2).to(DEV).double()[:, None]
+        y = b @ (w2[e].double() * s2[e].double()[:, None]).T
+        out.index_add_(0, token, y * weights[token, choice].double()[:, None])
+    return out
+
+
+def moe_case(tokens, hidden, inter, experts, choices, dtype=torch.bfloat16):
+    from harness import moe
+
+    g = rng_of(tokens + hidden)
+    w13, s13 = moe.quantize_int8_weights(torch.randn((experts, 2 * inter, hidden), device=DEV, generator=g) / hidden ** 0.5)
+    w2, s2 = moe.quantize_int8_weights(torch.randn((experts, hidden, inter), device=DEV, generator=g) / inter ** 0.5)
+    x = torch.randn((tokens, hidden), device=DEV, generator=g).to(dtype)
+    scores = torch.rand((tokens, experts), device=DEV, generator=g)
+    scores[:, experts - 1] = -1.0                   # an expert without tokens
+    weights, ids = torch.topk(scores, choices, dim=1)
+    return moe.Int8MoELayer(w13, s13, w2, s2), x, ids, weights
+
+
+def assert_moe(got, x, ids, weights, layer):
+    """Against the stages in 64 bits. A gate next to a rounding border of BF16 may land a step (2^-8
+    of its value) apart and take its code along: a code's step is 1/127 of the row's largest value.
+    Such values are rare (the gate's FP32 error is below 2^-19 of it, a step of BF16 2^-8: one in
+    2^10) and their effect on an output is one term of the sum: 2^-7 * |h| * |w2|. The output is
+    FP16 (2^-11 of its value) before the weighted FP32 sum. Rows are compared as vectors: the
+    error's norm is below (2^-11 + 2^-7 * sqrt(2^-10) + a hundred FP32 roundings) of the row's."""
+    want = moe_plain(x, ids, weights, layer.w13, layer.w13_scales, layer.w2, layer.w2_scales)
+    bound = 2.0 ** -11 + 2.0 ** -7 * 2.0 ** -5 + 100 * U
+    # The norm of a row's FP16 terms, not of their sum, is what the roundings are relative to.
+    size = want.norm(dim=1).max()
+    off = (got.double() - want).norm(dim=1)
+    assert (off <= 4 * bound * size).all(), (off / size).max().item()
+
+
+@pytest.mark.parametrize("tokens,hidden,inter,experts,choices,dtype", [
+    (1, 64, 32, 4, 2, torch.bfloat16), (33, 256, 96, 6, 2, torch.float32), (200, 512, 256, 8, 3, torch.float16),
+    (700, 256, 144, 5, 1, torch.bfloat16)])
+def test_int8_layer_against_its_stages(tokens, hidden, inter, experts, choices, dtype):
+    layer, x, ids, weights = moe_case(tokens, hidden, inter, experts, choices, dtype)
+    got = layer.forward(x, ids, weights)
+    assert got.shape == x.shape and got.dtype == torch.float32
+    assert_moe(got, x, ids, weights, layer)
+    assert torch.equal(got, layer.forward(x, ids.int(), weights))    # whatever the rows' order
+    ids[0, 0] = experts + 3                                          # no expert: adds nothing
+    dropped = weights.clone()
+    dropped[0, 0] = 0
+    ids_ok = ids.clone()
+    ids_ok[0, 0] = 0
+    assert torch.equal(layer.forward(x, ids, weights)[1:], layer.forward(x, ids_ok, dropped)[1:])
+    torch.testing.assert_close(layer.forward(x, ids, weights)[0], layer.forward(x, ids_ok, dropped)[0], rtol=0, atol=0)
+    assert layer.forward(x[:0], ids[:0], weights[:0]).shape == (0, hidden)
+    with pytest.raises(ValueError):
+        layer.forward(x[:, :-16], ids, weights)
+
+
+def test_int8_block_chain_in_a_graph():
+    """Two blocks, the first's last norm fused with the second's first, captured and replayed on new
+    tokens, equal the same operators called one by one."""
+    from harness import moe
+
+    tokens, hidden = 40, 256
+    layer, x, _, _ = moe_case(tokens, hidden, 96, 6, 2)
+    g = rng_of(77)
+    pre, post = (0.5 + torch.rand((2, hidden), device=DEV, generator=g) for _ in range(2))
+    gate = torch.randn((2, 4, hidden), device=DEV, generator=g)
+    router = torch.randn((hidden, 6), device=DEV, generator=g)
+    blocks = [moe.MoEBlock(layer, pre[i], post[i], gate[i], 0.7) for i in range(2)]
+
+    def route(n):
+        weights, ids = torch.topk(torch.softmax(n.float() @ router, dim=1), 2, dim=1)
+        return ids, weights
+
+    def chain(residual):
+        residual, normed = blocks[0].forward(residual, route, next_weight=pre[1])
+        return blocks[1].forward(residual, route, normed)[0]
+
+    static = x.clone()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        chain(static)
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = chain(static)
+    for seed in (1, 2):
+        fresh = torch.randn(x.shape, device=DEV, generator=rng_of(seed)).bfloat16()
+        static.copy_(fresh)
+        graph.replay()
+        want = fresh
+        for i in range(2):
+            n = int8.residual_norm(want, next_weight=pre[i])[1] if i == 0 else n
+            y = layer.forward(n, *route(n))
+            want, n, _ = int8.residual_norm(y, want, post_weight=post[i], gate=gate[i], residual_scale=0.7,
+                                            next_weight=pre[1] if i == 0 else None)
+        assert torch.equal(out, want)
+
+
+def test_block_around_the_fp4_layer():
+    """The norms serve the NVFP4 layers as well: the block equals norm, layer, norm."""
+    from harness import moe
+    from test_gpu_moe import quantised_weights, routing
+
+    device = torch.device(DEV)
+    w13, _, w13_blocked = quantised_weights(4, 256, 256, 1, device)
+    w2, _, w2_blocked = quantised_weights(4, 256, 128, 2, device)
+    layer = moe.RoutedMoELayer(w13, w13_blocked, w2, w2_blocked, max_pairs=128)
+    g = rng_of(5)
+    residual = torch.randn((50, 256), device=DEV, generator=g).bfloat16()
+    pre, post = 0.5 + torch.rand((2, 256), device=DEV, generator=g)
+    ids, weights = routing(50, 4, 2, 3, device)
+    got, normed = moe.MoEBlock(layer, pre, post).forward(residual, lambda n: (ids, weights), next_weight=pre)
+    n = int8.residual_norm(residual, next_weight=pre)[1]
+    y = layer.forward(n, ids, weights)
+    plain = norm_plain(y, residual, post, None, 1.0, pre, 1e-6)
+    assert_norm((got, normed, None), torch.bfloat16, torch.bfloat16, plain)
+    layer.close()

@@ -96,7 +96,8 @@ def test_entry_points_refuse_before_cuda(library):
     assert grouped(experts=0) == native.E_UNSUPPORTED_SHAPE
     assert grouped(experts=1025) == native.E_UNSUPPORTED_SHAPE
     assert grouped(stride=-256) == native.E_INVALID_ARGUMENT
-    assert grouped(stride=8) == native.E_MISALIGNED
+    assert grouped(stride=240) == native.E_INVALID_ARGUMENT      # experts overlap
+    assert grouped(stride=264) == native.E_MISALIGNED
     assert grouped(offsets=18) == native.E_MISALIGNED
     assert grouped(rows=0) == 0
 
