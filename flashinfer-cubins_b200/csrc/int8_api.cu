@@ -292,7 +292,16 @@ RowGrid row_grid(int rows, int width, int p, int elements) {
   g.elements = p == 8 && rows > 2 * host_sm_count() ? elements : 8;
   while ((width + g.elements - 1) / g.elements > 1024) g.elements *= 2;
   g.threads = ((width + g.elements - 1) / g.elements + 31) / 32 * 32;
-  if (p == 1) g.threads = g.threads <= 128 ? 128 : g.threads <= 256 ? 256 : g.threads <= 512 ? 512 : 1024;
+  if (p == 1) {  // the shapes that there are kernels for
+    if (g.elements > 8) {
+      g.threads = 1024;
+    } else if (g.threads > 768) {
+      g.elements = 16;
+      g.threads = 512;
+    } else {
+      g.threads = g.threads > 512 ? 768 : (g.threads + 127) / 128 * 128;
+    }
+  }
   g.blocks = rows;
   return g;
 }
@@ -304,15 +313,20 @@ void launch_quantize(const RowGrid& g, cudaStream_t s, const QuantizeParams& p) 
   if (g.warp) {
     kernel = g.elements == 8 ? int8_quantize_kernel<WIDE, P, 8 / P, kWarps, true>
                              : int8_quantize_kernel<WIDE, P, 32 / P, kWarps, true>;
-  } else if (P == 1 && g.threads < 1024) {
+  } else if constexpr (P == 1) {
     kernel = g.threads == 128   ? int8_quantize_kernel<WIDE, 1, 8, 128, false>
              : g.threads == 256 ? int8_quantize_kernel<WIDE, 1, 8, 256, false>
-                                : int8_quantize_kernel<WIDE, 1, 8, 512, false>;
+             : g.threads == 384 ? int8_quantize_kernel<WIDE, 1, 8, 384, false>
+             : g.threads == 768 ? int8_quantize_kernel<WIDE, 1, 8, 768, false>
+             : g.elements == 8  ? int8_quantize_kernel<WIDE, 1, 8, 512, false>
+             : g.threads == 512 ? int8_quantize_kernel<WIDE, 1, 16, 512, false>
+             : g.elements == 16 ? int8_quantize_kernel<WIDE, 1, 16, 1024, false>
+                                : int8_quantize_kernel<WIDE, 1, 32, 1024, false>;
   } else {
-    kernel = g.elements == 8    ? int8_quantize_kernel<WIDE, P, 8 / P, 1024, false>
-             : g.elements == 16 ? int8_quantize_kernel<WIDE, P, 16 / P, 1024, false>
-             : g.threads <= 512 ? int8_quantize_kernel<WIDE, P, 32 / P, 512, false>
-                                : int8_quantize_kernel<WIDE, P, 32 / P, 1024, false>;
+    kernel = g.elements == 8    ? int8_quantize_kernel<WIDE, 8, 1, 1024, false>
+             : g.elements == 16 ? int8_quantize_kernel<WIDE, 8, 2, 1024, false>
+             : g.threads <= 512 ? int8_quantize_kernel<WIDE, 8, 4, 512, false>
+                                : int8_quantize_kernel<WIDE, 8, 4, 1024, false>;
   }
   kernel<<<g.blocks, g.threads, 0, s>>>(p);
 }
@@ -324,15 +338,20 @@ void launch_norm(const RowGrid& g, cudaStream_t s, const NormParams& p) {
   if (g.warp) {
     kernel = g.elements == 8 ? residual_norm_kernel<X_WIDE, R_WIDE, P, 8 / P, kWarps, true>
                              : residual_norm_kernel<X_WIDE, R_WIDE, P, 32 / P, kWarps, true>;
-  } else if (P == 1 && g.threads < 1024) {
+  } else if constexpr (P == 1) {
     kernel = g.threads == 128   ? residual_norm_kernel<X_WIDE, R_WIDE, 1, 8, 128, false>
              : g.threads == 256 ? residual_norm_kernel<X_WIDE, R_WIDE, 1, 8, 256, false>
-                                : residual_norm_kernel<X_WIDE, R_WIDE, 1, 8, 512, false>;
+             : g.threads == 384 ? residual_norm_kernel<X_WIDE, R_WIDE, 1, 8, 384, false>
+             : g.threads == 768 ? residual_norm_kernel<X_WIDE, R_WIDE, 1, 8, 768, false>
+             : g.elements == 8  ? residual_norm_kernel<X_WIDE, R_WIDE, 1, 8, 512, false>
+             : g.threads == 512 ? residual_norm_kernel<X_WIDE, R_WIDE, 1, 16, 512, false>
+             : g.elements == 16 ? residual_norm_kernel<X_WIDE, R_WIDE, 1, 16, 1024, false>
+                                : residual_norm_kernel<X_WIDE, R_WIDE, 1, 32, 1024, false>;
   } else {
-    kernel = g.elements == 8    ? residual_norm_kernel<X_WIDE, R_WIDE, P, 8 / P, 1024, false>
-             : g.elements == 32 ? residual_norm_kernel<X_WIDE, R_WIDE, P, 32 / P, 1024, false>
-             : g.threads <= 512 ? residual_norm_kernel<X_WIDE, R_WIDE, P, 16 / P, 512, false>
-                                : residual_norm_kernel<X_WIDE, R_WIDE, P, 16 / P, 1024, false>;
+    kernel = g.elements == 8    ? residual_norm_kernel<X_WIDE, R_WIDE, 8, 1, 1024, false>
+             : g.elements == 32 ? residual_norm_kernel<X_WIDE, R_WIDE, 8, 4, 1024, false>
+             : g.threads <= 512 ? residual_norm_kernel<X_WIDE, R_WIDE, 8, 2, 512, false>
+                                : residual_norm_kernel<X_WIDE, R_WIDE, 8, 2, 1024, false>;
   }
   kernel<<<g.blocks, g.threads, 0, s>>>(p);
 }
@@ -413,7 +432,8 @@ int nvfp4_int8_quantize(const void* x, int x_kind, long long ldx, const int* sou
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (k > kMaxRegisterRow) {
     int8_quantize_long_kernel<<<rows, 1024, 0, s>>>(p);
-  } else if (rows_in_eights(x, ldx, kind_bytes(x_kind), tokens) && rows_in_eights(q, ldq, 1, rows)) {
+  } else if (k % 8 == 0 && rows_in_eights(x, ldx, kind_bytes(x_kind), tokens) &&
+             rows_in_eights(q, ldq, 1, rows)) {
     const RowGrid g = row_grid(rows, k, 8, 32);
     if (x_kind == NVFP4_IN_F32) launch_quantize<true, 8>(g, s, p); else launch_quantize<false, 8>(g, s, p);
   } else {
@@ -489,7 +509,8 @@ int nvfp4_residual_norm(const void* x, int x_kind, long long ldx, const void* re
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int y_bytes = y_kind == NVFP4_NORM_CODES ? 1 : kind_bytes(y_kind);
   const int r_bytes = static_cast<int>(residual_bytes);
-  if (rows_in_eights(x, ldx, kind_bytes(x_kind), tokens) && rows_in_eights(residual, ldres, r_bytes, tokens) &&
+  if (hidden % 8 == 0 && rows_in_eights(x, ldx, kind_bytes(x_kind), tokens) &&
+      rows_in_eights(residual, ldres, r_bytes, tokens) &&
       rows_in_eights(r, ldr, r_bytes, tokens) && rows_in_eights(post_weight, 0, 4, 1) &&
       rows_in_eights(gate, hidden, 4, gates) &&
       (next_weight == nullptr || (rows_in_eights(next_weight, 0, 4, 1) && rows_in_eights(y, ldy, y_bytes, tokens)))) {

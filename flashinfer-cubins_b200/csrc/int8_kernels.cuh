@@ -147,9 +147,9 @@ __device__ __forceinline__ int one_code(float v, const RowCodes& row) {
 //
 // A row belongs to one warp (WARP: eight rows to a CTA, no barrier) or to one CTA, whose threads
 // hold N pieces of P neighbouring elements each, read once, every load issued before the first is
-// used. P = 8 where all rows start on a multiple of eight elements: 16-byte loads of 16-bit
-// elements, 32-byte ones of 32-bit elements (two 16-byte loads a lane, 32 bytes apart, took the L1
-// cache twice the cycles), and a last piece that may be short. P = 1 for any other start and pitch:
+// used. P = 8 where all rows start on a multiple of eight elements and are a multiple of eight long:
+// 16-byte loads of 16-bit elements, 32-byte ones of 32-bit elements (two 16-byte loads a lane, 32
+// bytes apart, took the L1 cache twice the cycles). P = 1 for any other start, pitch and length:
 // there the CTA has its full THREADS, so that a thread's elements lie constant distances apart and
 // an access needs no address of its own (8192 x 5121 norms: 319 us with computed addresses).
 
@@ -172,43 +172,25 @@ struct Raw {
   uint32_t w[kWords];
 };
 
-// Elements c .. c + P - 1 of a row of which `left` are there; zero beyond them.
+// Elements c .. c + P - 1 of a row of `width`; zero if they lie beyond it.
 template <bool WIDE, int P>
-__device__ __forceinline__ Raw<WIDE, P> load_raw(const void* row, int c, int left) {
-  Raw<WIDE, P> r;
-  if constexpr (P == 1) {
-    r.w[0] = 0;
-    if (left > 0) {
+__device__ __forceinline__ Raw<WIDE, P> load_raw(const void* row, int c, int width) {
+  Raw<WIDE, P> r{};
+  if (c < width) {
+    if constexpr (P == 1) {
       if constexpr (WIDE) {
         r.w[0] = static_cast<const uint32_t*>(row)[c];
       } else {
         r.w[0] = static_cast<const uint16_t*>(row)[c];
       }
-    }
-  } else {
-    if (left >= 8) {
-      if constexpr (WIDE) {
-        load_32_bytes(static_cast<const float*>(row) + c, r.w);
-      } else {
-        const uint4 q = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(row) + c);
-        r.w[0] = q.x;
-        r.w[1] = q.y;
-        r.w[2] = q.z;
-        r.w[3] = q.w;
-      }
+    } else if constexpr (WIDE) {
+      load_32_bytes(static_cast<const float*>(row) + c, r.w);
     } else {
-#pragma unroll
-      for (int i = 0; i < Raw<WIDE, P>::kWords; ++i) r.w[i] = 0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (i < left) {
-          if constexpr (WIDE) {
-            r.w[i] = static_cast<const uint32_t*>(row)[c + i];
-          } else {
-            r.w[i / 2] |= static_cast<uint32_t>(static_cast<const uint16_t*>(row)[c + i]) << (16 * (i % 2));
-          }
-        }
-      }
+      const uint4 q = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(row) + c);
+      r.w[0] = q.x;
+      r.w[1] = q.y;
+      r.w[2] = q.z;
+      r.w[3] = q.w;
     }
   }
   return r;
@@ -235,68 +217,60 @@ __device__ __forceinline__ void unpack(const Raw<WIDE, P>& r, bool half, float (
 
 // FP32 values of a vector over the row (weights, gates), zero beyond it.
 template <int P>
-__device__ __forceinline__ void load_weights(const float* row, int c, int left, float (&v)[P]) {
-  unpack<true, P>(load_raw<true, P>(row, c, left), false, v);
+__device__ __forceinline__ void load_weights(const float* row, int c, int width, float (&v)[P]) {
+  unpack<true, P>(load_raw<true, P>(row, c, width), false, v);
 }
 
 // Stores values of kind NVFP4_IN_*.
 template <int P>
-__device__ __forceinline__ void store_values(void* row, int c, int left, int kind, const float (&v)[P]) {
+__device__ __forceinline__ void store_values(void* row, int c, int kind, const float (&v)[P]) {
   if (kind == 0) {
     float* p = static_cast<float*>(row) + c;
     if constexpr (P == 8) {
-      if (left >= 8) {
-        store_32_bytes(p, v);
-        return;
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < P; ++i) {
-      if (i < left) p[i] = v[i];
+      store_32_bytes(p, v);
+    } else {
+      p[0] = v[0];
     }
     return;
   }
-  uint32_t w[(P + 1) / 2];
-#pragma unroll
-  for (int i = 0; i < (P + 1) / 2; ++i) {
-    const float low = v[2 * i], high = 2 * i + 1 < P ? v[(2 * i + 1) % P] : 0.0f;
-    if (kind == 1) {
-      const __nv_bfloat162 b = __floats2bfloat162_rn(low, high);
-      w[i] = *reinterpret_cast<const uint32_t*>(&b);
-    } else {
-      const __half2 b = __floats2half2_rn(low, high);
-      w[i] = *reinterpret_cast<const uint32_t*>(&b);
-    }
-  }
   uint16_t* p = static_cast<uint16_t*>(row) + c;
   if constexpr (P == 8) {
-    if (left >= 8) {
-      *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
-      return;
-    }
-  }
+    uint32_t w[4];
+    if (kind == 1) {
 #pragma unroll
-  for (int i = 0; i < P; ++i) {
-    if (i < left) p[i] = static_cast<uint16_t>(w[i / 2] >> (16 * (i % 2)));
+      for (int i = 0; i < 4; ++i) {
+        const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&b);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const __half2 b = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&b);
+      }
+    }
+    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+  } else if (kind == 1) {
+    *reinterpret_cast<__nv_bfloat16*>(p) = from_float<__nv_bfloat16>(v[0]);
+  } else {
+    *reinterpret_cast<__half*>(p) = from_float<__half>(v[0]);
   }
 }
 
 // Codes of P values.
 template <int P>
-__device__ __forceinline__ void store_codes(int8_t* row, int c, int left, const float (&v)[P], const RowCodes& codes) {
+__device__ __forceinline__ void store_codes(int8_t* row, int c, const float (&v)[P], const RowCodes& codes) {
   if constexpr (P == 8) {
-    const uint2 b = eight_codes(v, codes);
-    if (left >= 8) {
-      *reinterpret_cast<uint2*>(row + c) = b;
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (i < left) row[c + i] = static_cast<int8_t>((i < 4 ? b.x : b.y) >> (8 * (i % 4)));
-      }
-    }
+    *reinterpret_cast<uint2*>(row + c) = eight_codes(v, codes);
   } else {
-    if (left > 0) row[c] = static_cast<int8_t>(one_code(v[0], codes));
+    row[c] = static_cast<int8_t>(one_code(v[0], codes));
   }
+}
+
+// CTAs that an SM is to hold: of rows taken one element at a time, 1,536 threads' worth (few registers,
+// and more rows under way: 8192 x 5121 norms 251 us with one CTA of 1,024 threads).
+constexpr int ctas_per_sm(int p, int n, int threads) {
+  return p != 1 || threads >= 1024 ? 1 : n == 8 ? 1536 / threads : n == 16 ? 1024 / threads : 1;
 }
 
 // Over the row's threads; `shared` (one word for each warp) serves one reduction of a kernel.
@@ -315,15 +289,10 @@ __device__ __forceinline__ double row_sum(double v, double* shared) {
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, d);
   if constexpr (WARP) return v;
-  const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  const int lane = threadIdx.x & 31;
   if (lane == 0) shared[threadIdx.x >> 5] = v;
   __syncthreads();
-  if (warps <= 12) {
-    v = shared[0];
-    for (int w = 1; w < warps; ++w) v += shared[w];
-    return v;
-  }
-  v = lane < warps ? shared[lane] : 0.0;
+  v = lane < static_cast<int>(blockDim.x >> 5) ? shared[lane] : 0.0;
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, d);
   return v;
@@ -350,7 +319,7 @@ struct QuantizeParams {
 // Row r of the codes = row source[r] (or r) of x. A source row outside [0, tokens) leaves the
 // row's codes and its scale as they were.
 template <bool WIDE, int P, int N, int THREADS, bool WARP>
-__global__ void __launch_bounds__(THREADS) int8_quantize_kernel(const QuantizeParams p) {
+__global__ void __launch_bounds__(THREADS, ctas_per_sm(P, N, THREADS)) int8_quantize_kernel(const QuantizeParams p) {
   __shared__ uint32_t maxima[32];
   const int r = row_of_thread<WARP>();
   if (r >= p.rows) return;
@@ -361,7 +330,7 @@ __global__ void __launch_bounds__(THREADS) int8_quantize_kernel(const QuantizePa
   const void* in = static_cast<const uint8_t*>(p.x) + t * p.ldx * (WIDE ? 4 : 2);
   Raw<WIDE, P> raw[N];
 #pragma unroll
-  for (int j = 0; j < N; ++j) raw[j] = load_raw<WIDE, P>(in, first + step * j, p.k - first - step * j);
+  for (int j = 0; j < N; ++j) raw[j] = load_raw<WIDE, P>(in, first + step * j, p.k);
   // 16-bit magnitudes order like their bits, too: the largest of the negative ones is the largest
   // unsigned pattern, that of the positive ones the largest signed one.
   uint32_t amax = 0, positive = 0;
@@ -393,7 +362,7 @@ __global__ void __launch_bounds__(THREADS) int8_quantize_kernel(const QuantizePa
     if (c < p.k) {
       float v[P];
       unpack<WIDE, P>(raw[j], half, v);
-      store_codes<P>(out, c, p.k - c, v, row);
+      store_codes<P>(out, c, v, row);
     }
   }
   if (first == 0) p.scales[r] = row.scale;
@@ -491,7 +460,7 @@ __device__ __forceinline__ void add(float (&v)[P], const float (&w)[P]) {
 }
 
 template <bool X_WIDE, bool R_WIDE, int P, int N, int THREADS, bool WARP>
-__global__ void __launch_bounds__(THREADS) residual_norm_kernel(const NormParams p) {
+__global__ void __launch_bounds__(THREADS, ctas_per_sm(P, N, THREADS)) residual_norm_kernel(const NormParams p) {
   __shared__ double post_sums[32], next_sums[32];
   __shared__ uint32_t maxima[32];
   const int t = row_of_thread<WARP>();
@@ -504,13 +473,13 @@ __global__ void __launch_bounds__(THREADS) residual_norm_kernel(const NormParams
   const void* x_row = row_at(p.x, t * p.ldx, p.x_kind);
 #pragma unroll
   for (int j = 0; j < N; ++j) {
-    raw_x[j] = load_raw<X_WIDE, P>(x_row, first + step * j, hidden - first - step * j);
+    raw_x[j] = load_raw<X_WIDE, P>(x_row, first + step * j, hidden);
   }
   if (p.residual != nullptr) {
     const void* res_row = row_at(p.residual, t * p.ldres, p.residual_kind);
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      raw_r[j] = load_raw<R_WIDE, P>(res_row, first + step * j, hidden - first - step * j);
+      raw_r[j] = load_raw<R_WIDE, P>(res_row, first + step * j, hidden);
     }
   }
   float v[N][P];
@@ -524,7 +493,7 @@ __global__ void __launch_bounds__(THREADS) residual_norm_kernel(const NormParams
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       float w[P];
-      load_weights<P>(p.post_weight, first + step * j, hidden - first - step * j, w);
+      load_weights<P>(p.post_weight, first + step * j, hidden, w);
       scale_by(v[j], rstd);
       multiply(v[j], w);
     }
@@ -534,7 +503,7 @@ __global__ void __launch_bounds__(THREADS) residual_norm_kernel(const NormParams
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       float g[P];
-      load_weights<P>(gate, first + step * j, hidden - first - step * j, g);
+      load_weights<P>(gate, first + step * j, hidden, g);
       multiply(v[j], g);
     }
   }
@@ -548,7 +517,7 @@ __global__ void __launch_bounds__(THREADS) residual_norm_kernel(const NormParams
 #pragma unroll
       for (int i = 0; i < P; ++i) res[i] = __fmul_rn(res[i], p.residual_scale);
       add(v[j], res);
-      if (c < hidden) store_values<P>(r_row, c, hidden - c, p.residual_kind, v[j]);
+      if (c < hidden) store_values<P>(r_row, c, p.residual_kind, v[j]);
     }
   }
   if (p.next_weight == nullptr) return;
@@ -559,7 +528,7 @@ __global__ void __launch_bounds__(THREADS) residual_norm_kernel(const NormParams
 #pragma unroll
   for (int j = 0; j < N; ++j) {
     float w[P];
-    load_weights<P>(p.next_weight, first + step * j, hidden - first - step * j, w);
+    load_weights<P>(p.next_weight, first + step * j, hidden, w);
     scale_by(v[j], rstd);
     multiply(v[j], w);
   }
@@ -568,7 +537,7 @@ __global__ void __launch_bounds__(THREADS) residual_norm_kernel(const NormParams
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       const int c = first + step * j;
-      if (c < hidden) store_values<P>(y_row, c, hidden - c, p.y_kind, v[j]);
+      if (c < hidden) store_values<P>(y_row, c, p.y_kind, v[j]);
     }
     return;
   }
@@ -583,7 +552,7 @@ __global__ void __launch_bounds__(THREADS) residual_norm_kernel(const NormParams
 #pragma unroll
   for (int j = 0; j < N; ++j) {
     const int c = first + step * j;
-    if (c < hidden) store_codes<P>(y_row, c, hidden - c, v[j], row);
+    if (c < hidden) store_codes<P>(y_row, c, v[j], row);
   }
   if (first == 0) p.scales[t] = row.scale;
 }

@@ -89,8 +89,9 @@ def _vector(t: torch.Tensor, shape: tuple, what: str, index: int) -> int:
 def empty_codes(rows: int, k: int, device: torch.device | str) -> torch.Tensor:
     """An INT8 ``[rows, k]`` buffer whose rows lie 16-byte aligned."""
     pitch = -(-k // 16) * 16
-    codes = torch.empty((rows, pitch), dtype=torch.int8, device=device)
-    return codes if pitch == k else codes[:, :k]
+    if pitch == k:
+        return torch.empty(rows, k, dtype=torch.int8, device=device)
+    return torch.empty(rows, pitch, dtype=torch.int8, device=device)[:, :k]
 
 
 def _codes(t: torch.Tensor, dims: int, what: str, index: int) -> int:
@@ -136,7 +137,7 @@ def gemm(a: torch.Tensor, b: torch.Tensor, a_scales: torch.Tensor, b_scales: tor
     pbias = None if bias is None else _vector(bias, (width,), "bias", index)
     _check_device(index)
     if out is None:
-        out, ldd = torch.empty((m, n), dtype=out_dtype, device=a.device), n
+        out, ldd = torch.empty(m, n, dtype=out_dtype, device=a.device), n
     else:
         ldd = _given(out, (m, n), out_dtype, index, "out")
     _launch(index, "nvfp4_int8_gemm", a.data_ptr(), lda, b.data_ptr(), ldb, pa, pb, pbias,
@@ -172,7 +173,7 @@ def grouped_gemm(a: torch.Tensor, b: torch.Tensor, a_scales: torch.Tensor, b_sca
                          f"got {offsets.dtype} {tuple(offsets.shape)} on {offsets.device}")
     _check_device(index)
     if out is None:
-        out, ldd = torch.empty((rows, n), dtype=out_dtype, device=a.device), n
+        out, ldd = torch.empty(rows, n, dtype=out_dtype, device=a.device), n
     else:
         ldd = _given(out, (rows, n), out_dtype, index, "out")
     _launch(index, "nvfp4_int8_group_gemm", a.data_ptr(), lda, b.data_ptr(), ldb,
@@ -208,7 +209,7 @@ def quantize_tokens(x: torch.Tensor, *, rows: torch.Tensor | None = None,
         device = x.device
         ldq = -(-k // 16) * 16
         q = empty_codes(count, k, device)
-        scales = torch.empty((count,), dtype=torch.float32, device=device)
+        scales = torch.empty(count, dtype=torch.float32, device=device)
         ps = scales.data_ptr()
     else:
         q, scales = out
@@ -270,7 +271,7 @@ def residual_norm(x: torch.Tensor, residual: torch.Tensor | None = None, *,
     r, pr, ldr = None, None, 0
     if residual is not None:
         if residual_out is None:
-            r, ldr = torch.empty(shape, dtype=residual.dtype, device=device), hidden
+            r, ldr = torch.empty(tokens, hidden, dtype=residual.dtype, device=device), hidden
         else:
             r, ldr = residual_out, _given(residual_out, shape, residual.dtype, index, "residual_out")
         pr = r.data_ptr()
@@ -278,14 +279,14 @@ def residual_norm(x: torch.Tensor, residual: torch.Tensor | None = None, *,
     if next_weight is not None:
         if quantize:
             y, ldy = empty_codes(tokens, hidden, device), -(-hidden // 16) * 16
-            scales = torch.empty((tokens,), dtype=torch.float32, device=device)
+            scales = torch.empty(tokens, dtype=torch.float32, device=device)
             pscales = scales.data_ptr()
         else:
             dtype = out_dtype or (x if residual is None else residual).dtype
             y_kind = IN_KINDS.get(dtype)
             if y_kind is None:
                 raise ValueError(f"no output in {dtype}")
-            y, ldy = torch.empty(shape, dtype=dtype, device=device), hidden
+            y, ldy = torch.empty(tokens, hidden, dtype=dtype, device=device), hidden
         py = y.data_ptr()
     _launch(index, "nvfp4_residual_norm", x.data_ptr(), x_kind, ldx, pres, kind, ldres, ppost, pgate, gates,
             residual_scale, pnext, eps, pr, ldr, py, y_kind, ldy, pscales, tokens, hidden)
