@@ -268,6 +268,25 @@ int launch_product(const Product& q, void* stream) {
   return 0;
 }
 
+// Launches a row kernel with programmatic stream serialization: its blocks may take their places while
+// the kernel before it ends (they wait on the device before they touch memory), and it lets the next
+// one do so.
+template <class Params>
+void launch_rows(void (*kernel)(Params), int blocks, int threads, cudaStream_t stream, Params p) {
+  cudaLaunchAttribute attribute[1];
+  attribute[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attribute[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(static_cast<unsigned int>(blocks));
+  config.blockDim = dim3(static_cast<unsigned int>(threads));
+  config.stream = stream;
+  config.attrs = attribute;
+  config.numAttrs = 1;
+  void* args[1] = {&p};
+  // An error is the launch's own and reported by the caller's cudaGetLastError().
+  (void)cudaLaunchKernelExC(&config, reinterpret_cast<const void*>(kernel), args);
+}
+
 // How rows of `width` elements lie over threads. A warp to a row up to 1,024 elements, where there
 // are rows enough; else a CTA. In pieces of eight: few threads with much work where there are many
 // rows (`elements` a thread: fewer, and the fixed cost of a row's reductions shows), many threads
@@ -328,7 +347,7 @@ void launch_quantize(const RowGrid& g, cudaStream_t s, const QuantizeParams& p) 
              : g.threads <= 512 ? int8_quantize_kernel<WIDE, 8, 4, 512, false>
                                 : int8_quantize_kernel<WIDE, 8, 4, 1024, false>;
   }
-  kernel<<<g.blocks, g.threads, 0, s>>>(p);
+  launch_rows(kernel, g.blocks, g.threads, s, p);
 }
 
 template <bool X_WIDE, bool R_WIDE, int P>
@@ -353,7 +372,7 @@ void launch_norm(const RowGrid& g, cudaStream_t s, const NormParams& p) {
              : g.threads <= 512 ? residual_norm_kernel<X_WIDE, R_WIDE, 8, 2, 512, false>
                                 : residual_norm_kernel<X_WIDE, R_WIDE, 8, 2, 1024, false>;
   }
-  kernel<<<g.blocks, g.threads, 0, s>>>(p);
+  launch_rows(kernel, g.blocks, g.threads, s, p);
 }
 
 template <int P>

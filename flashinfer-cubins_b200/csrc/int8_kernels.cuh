@@ -321,6 +321,8 @@ struct QuantizeParams {
 template <bool WIDE, int P, int N, int THREADS, bool WARP>
 __global__ void __launch_bounds__(THREADS, ctas_per_sm(P, N, THREADS)) int8_quantize_kernel(const QuantizeParams p) {
   __shared__ uint32_t maxima[32];
+  grid_dependency_wait();
+  grid_launch_dependents();
   const int r = row_of_thread<WARP>();
   if (r >= p.rows) return;
   const int t = p.source != nullptr ? __ldg(p.source + r) : r;
@@ -463,6 +465,8 @@ template <bool X_WIDE, bool R_WIDE, int P, int N, int THREADS, bool WARP>
 __global__ void __launch_bounds__(THREADS, ctas_per_sm(P, N, THREADS)) residual_norm_kernel(const NormParams p) {
   __shared__ double post_sums[32], next_sums[32];
   __shared__ uint32_t maxima[32];
+  grid_dependency_wait();
+  grid_launch_dependents();
   const int t = row_of_thread<WARP>();
   if (t >= p.tokens) return;
   const int hidden = p.hidden;
