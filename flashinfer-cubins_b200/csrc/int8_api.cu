@@ -44,6 +44,8 @@ bool is_in_kind(int kind) {
 // Sums of k products of two codes of -128..127 stay below 2^31 up to here.
 constexpr int kMaxDepth = 131071;
 constexpr int kMaxHidden = 32768;
+// Rows of A, and of B: sums of a tile's rows stay within 32 bits.
+constexpr int kMaxRows = 1 << 30;
 
 // One product, dense (offsets null, one expert) or grouped.
 struct Product {
@@ -60,7 +62,7 @@ struct Product {
 };
 
 int check_product(const Product& p) {
-  if (p.rows < 0 || p.n < 1 || p.n > (1 << 30) || p.k < 1 || p.k > kMaxDepth || p.experts < 1 ||
+  if (p.rows < 0 || p.rows > kMaxRows || p.n < 1 || p.n > (p.gated ? kMaxRows / 2 : kMaxRows) || p.k < 1 || p.k > kMaxDepth || p.experts < 1 ||
       p.experts > kInt8MaxExperts) {
     return fail(NVFP4_E_UNSUPPORTED_SHAPE,
                 "unsupported product: %d rows, n=%d, k=%d (at most %d), %d experts (at most %d)",
@@ -310,6 +312,7 @@ RowGrid row_grid(int rows, int width, int p, int elements) {
   }
   g.elements = p == 8 && rows > 2 * host_sm_count() ? elements : 8;
   while ((width + g.elements - 1) / g.elements > 1024) g.elements *= 2;
+  // One CTA of 1,024 threads on an SM is one row under way: two of 512 with twice the work.
   g.threads = ((width + g.elements - 1) / g.elements + 31) / 32 * 32;
   if (p == 1) {  // the shapes that there are kernels for
     if (g.elements > 8) {
@@ -368,7 +371,8 @@ void launch_norm(const RowGrid& g, cudaStream_t s, const NormParams& p) {
                                 : residual_norm_kernel<X_WIDE, R_WIDE, 1, 32, 1024, false>;
   } else {
     kernel = g.elements == 8    ? residual_norm_kernel<X_WIDE, R_WIDE, 8, 1, 1024, false>
-             : g.elements == 32 ? residual_norm_kernel<X_WIDE, R_WIDE, 8, 4, 1024, false>
+             : g.elements == 32 ? (g.threads <= 512 ? residual_norm_kernel<X_WIDE, R_WIDE, 8, 4, 512, false>
+                                                    : residual_norm_kernel<X_WIDE, R_WIDE, 8, 4, 1024, false>)
              : g.threads <= 512 ? residual_norm_kernel<X_WIDE, R_WIDE, 8, 2, 512, false>
                                 : residual_norm_kernel<X_WIDE, R_WIDE, 8, 2, 1024, false>;
   }

@@ -104,7 +104,7 @@ __device__ __forceinline__ RowCodes row_codes(uint32_t amax_bits) {
 // quotient (|q| <= 127), so where it lies more than 2^-15 from the middle between two integers the
 // quotient, rounded, lies on the same side. Adding 1.5 * 2^23 rounds it to an integer (ties to even)
 // whose low byte is the code. Values nearer to a middle (one in 2^14) are divided. Dividing all of
-// them cost 94 us for 8192 x 7168 BF16 values, this 35.
+// them cost 94 us for 8192 x 7168 BF16 values, this 32.
 constexpr float kRoundBias = 12582912.0f;
 
 __device__ __forceinline__ bool near_middle(float off) { return off >= 0.5f - 0x1p-15f; }
@@ -267,10 +267,17 @@ __device__ __forceinline__ void store_codes(int8_t* row, int c, const float (&v)
   }
 }
 
-// CTAs that an SM is to hold: of rows taken one element at a time, 1,536 threads' worth (few registers,
-// and more rows under way: 8192 x 5121 norms 251 us with one CTA of 1,024 threads).
-constexpr int ctas_per_sm(int p, int n, int threads) {
-  return p != 1 || threads >= 1024 ? 1 : n == 8 ? 1536 / threads : n == 16 ? 1024 / threads : 1;
+// Registers of a thread. What bounds the row kernels is how many rows are under way on an SM (half of
+// the issue slots idle with three), so they get fewer than the compiler would take: the norms in pieces
+// of eight 48 (8192 x 5120: 70 us, with 64 registers 78, with 40 and spills 73), the quantiser 40 (8192 x
+// 7168: 31.8 us, with 52 registers 32.4), rows taken one element at a time 40 (4096 x 3001 to codes: 43
+// us, with 64 registers 53). CTAs of 1,024 threads and threads of 32 single elements need 64.
+constexpr int row_registers(bool norm, int p, int n, int threads, bool warp) {
+  const int elements = p * n;
+  if (elements == 8) return p == 1 ? 40 : threads == 1024 ? 64 : 48;
+  if (warp) return norm ? 64 : 48;
+  if (p == 8 && threads == 512) return !norm ? 40 : n == 2 ? 48 : 64;
+  return 64;
 }
 
 // Over the row's threads; `shared` (one word for each warp) serves one reduction of a kernel.
@@ -319,7 +326,7 @@ struct QuantizeParams {
 // Row r of the codes = row source[r] (or r) of x. A source row outside [0, tokens) leaves the
 // row's codes and its scale as they were.
 template <bool WIDE, int P, int N, int THREADS, bool WARP>
-__global__ void __launch_bounds__(THREADS, ctas_per_sm(P, N, THREADS)) int8_quantize_kernel(const QuantizeParams p) {
+__global__ void __maxnreg__(row_registers(false, P, N, THREADS, WARP)) int8_quantize_kernel(const QuantizeParams p) {
   __shared__ uint32_t maxima[32];
   grid_dependency_wait();
   grid_launch_dependents();
@@ -462,7 +469,7 @@ __device__ __forceinline__ void add(float (&v)[P], const float (&w)[P]) {
 }
 
 template <bool X_WIDE, bool R_WIDE, int P, int N, int THREADS, bool WARP>
-__global__ void __launch_bounds__(THREADS, ctas_per_sm(P, N, THREADS)) residual_norm_kernel(const NormParams p) {
+__global__ void __maxnreg__(row_registers(true, P, N, THREADS, WARP)) residual_norm_kernel(const NormParams p) {
   __shared__ double post_sums[32], next_sums[32];
   __shared__ uint32_t maxima[32];
   grid_dependency_wait();

@@ -823,13 +823,36 @@ int create_dense_like(nvfp4_plan** out, int kind, int device, int out_kind, int 
 // What the other translation units of the library use of this one (nvfp4_host.h).
 namespace nvfp4 {
 
-int host_fail(int code, const char* text) noexcept { return fail(code, "%s", text); }
+int host_fail(int code, const char* text) noexcept {
+  try {
+    g_last_error = text;
+  } catch (...) {  // no memory for the text: the code is returned all the same
+  }
+  return code;
+}
 
-int host_fail_cuda(cudaError_t error, const char* what) noexcept { return fail_cuda(error, what); }
+int host_fail_cuda(cudaError_t error, const char* what) noexcept {
+  cudaGetLastError();
+  char text[384];
+  snprintf(text, sizeof(text), "%s: %s", what, cudaGetErrorString(error));
+  return host_fail(static_cast<int>(error), text);
+}
 
-int host_encoder(EncodeTiled* out) noexcept { return get_encoder(out); }
+int host_encoder(EncodeTiled* out) noexcept {
+  try {
+    return get_encoder(out);
+  } catch (...) {
+    return host_fail(NVFP4_E_INVALID_ARGUMENT, "the tensor-map encoder cannot be looked up");
+  }
+}
 
-int host_sm_count() noexcept { return current_sm_count(); }
+int host_sm_count() noexcept {
+  try {
+    return current_sm_count();
+  } catch (...) {
+    return 148;
+  }
+}
 
 }  // namespace nvfp4
 

@@ -34,9 +34,12 @@ IN_KINDS = {torch.float32: native.IN_F32, torch.bfloat16: native.IN_BF16,
 MAX_DEPTH = 131071  # k: sums of products of codes stay within 32 bits
 MAX_EXPERTS = 1024
 MAX_HIDDEN = 32768
+MAX_ROWS = 1 << 30  # rows of an operand; n at most half of that
 
 # Decode calls take a few microseconds on the GPU, so the host's share counts: devices are compared by
-# index, and the current stream's handle is read without making a Stream object (2 us less).
+# index, the current stream's handle is read without making a Stream object (2 us), and a tensor's
+# checks are one function call.
+_INT8, _FLOAT = torch.int8, torch.float32
 _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 _supported: dict[int, bool] = {}
@@ -69,18 +72,28 @@ def _refuse_gradients(*tensors) -> None:
             raise ValueError("the INT8 operators have no backward; call them under torch.no_grad()")
 
 
-def _pitch(t: torch.Tensor, what: str) -> int:
-    """Elements between the rows of ``t`` (its last but one dimension)."""
-    shape = t.shape
+def check_status(device: torch.device | str | int | None = None) -> None:
+    """Synchronise ``device``'s current stream and raise ``native.NativeError`` if a product on it
+    abandoned a bounded wait since the last call (its result is then undefined)."""
+    with torch.cuda.device(device):
+        value = native.ctypes.c_int(0)
+        native.check(native.load().nvfp4_int8_status(_raw_stream(torch.cuda.current_device()),
+                                                     native.ctypes.byref(value)))
+
+
+def _too_many(what: str, count: int) -> None:
+    raise ValueError(f"{what}: {count} rows, at most {MAX_ROWS}")
+
+
+def _rows(t: torch.Tensor, shape, what: str) -> int:
+    """Elements between the rows of ``t`` (its last but one dimension; ``shape`` is its shape)."""
     if shape[-1] > 1 and t.stride(-1) != 1:
         raise ValueError(f"{what}: elements of a row must be neighbours")
-    if shape[-2] > 1:
-        return t.stride(-2)
-    return -(-shape[-1] // 16) * 16  # one row: nothing lies between
+    return t.stride(-2) if shape[-2] > 1 else -(-shape[-1] // 16) * 16  # one row: nothing lies between
 
 
 def _vector(t: torch.Tensor, shape: tuple, what: str, index: int) -> int:
-    if t.dtype is not torch.float32 or t.shape != shape or not t.is_contiguous() or t.get_device() != index:
+    if t.dtype is not _FLOAT or t.shape != shape or not t.is_contiguous() or t.get_device() != index:
         raise ValueError(f"{what}: expected contiguous float32 {shape} beside the first operand, got "
                          f"{t.dtype} {tuple(t.shape)} on {t.device}")
     return t.data_ptr()
@@ -95,10 +108,13 @@ def empty_codes(rows: int, k: int, device: torch.device | str) -> torch.Tensor:
 
 
 def _codes(t: torch.Tensor, dims: int, what: str, index: int) -> int:
-    if t.dtype is not torch.int8 or t.dim() != dims or t.get_device() != index:
+    shape = t.shape
+    if t.dtype is not _INT8 or len(shape) != dims or t.get_device() != index:
         raise ValueError(f"{what}: expected {dims}-d int8 beside the first operand, got {t.dtype} "
-                         f"{tuple(t.shape)} on {t.device}")
-    return _pitch(t, what)
+                         f"{tuple(shape)} on {t.device}")
+    if shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{what}: elements of a row must be neighbours")
+    return t.stride(-2) if shape[-2] > 1 else -(-shape[-1] // 16) * 16
 
 
 def _given(out: torch.Tensor, shape: tuple, dtype: torch.dtype, index: int, what: str) -> int:
@@ -106,7 +122,7 @@ def _given(out: torch.Tensor, shape: tuple, dtype: torch.dtype, index: int, what
     if out.dtype is not dtype or out.shape != shape or out.get_device() != index:
         raise ValueError(f"{what}: expected {dtype} {shape} beside the first operand, got {out.dtype} "
                          f"{tuple(out.shape)} on {out.device}")
-    return _pitch(out, what)
+    return _rows(out, shape, what)
 
 
 def _width(width: int, gated: bool) -> int:
@@ -129,6 +145,8 @@ def gemm(a: torch.Tensor, b: torch.Tensor, a_scales: torch.Tensor, b_scales: tor
     (m, k), (width, depth) = a.shape, b.shape
     if depth != k:
         raise ValueError(f"a is {k} deep, b {depth}")
+    if m > MAX_ROWS or width > MAX_ROWS:
+        _too_many("a or b", max(m, width))
     kind = OUT_KINDS.get(out_dtype)
     if kind is None:
         raise ValueError(f"no output in {out_dtype}")
@@ -161,6 +179,8 @@ def grouped_gemm(a: torch.Tensor, b: torch.Tensor, a_scales: torch.Tensor, b_sca
     (rows, k), (experts, width, depth) = a.shape, b.shape
     if depth != k:
         raise ValueError(f"a is {k} deep, b {depth}")
+    if rows > MAX_ROWS or width > MAX_ROWS:
+        _too_many("a or b", max(rows, width))
     kind = OUT_KINDS.get(out_dtype)
     if kind is None:
         raise ValueError(f"no output in {out_dtype}")
@@ -196,7 +216,7 @@ def quantize_tokens(x: torch.Tensor, *, rows: torch.Tensor | None = None,
     kind = IN_KINDS.get(x.dtype)
     if x.dim() != 2 or kind is None:
         raise ValueError(f"x: expected 2-d FP32, BF16 or FP16, got {x.dtype} {tuple(x.shape)}")
-    ldx = _pitch(x, "x")
+    ldx = _rows(x, x.shape, "x")
     tokens, k = x.shape
     count, source = tokens, None
     if rows is not None:
@@ -204,6 +224,8 @@ def quantize_tokens(x: torch.Tensor, *, rows: torch.Tensor | None = None,
             raise ValueError(f"rows: expected contiguous 1-d int32 beside the first operand, got {rows.dtype} "
                              f"{tuple(rows.shape)} on {rows.device}")
         count, source = rows.numel(), rows.data_ptr()
+    if max(tokens, count, k) > MAX_ROWS:
+        _too_many("x", max(tokens, count, k))
     _check_device(index)
     if out is None:
         device = x.device
@@ -246,20 +268,24 @@ def residual_norm(x: torch.Tensor, residual: torch.Tensor | None = None, *,
         raise ValueError(f"x: expected 2-d FP32, BF16 or FP16, got {x.dtype} {tuple(x.shape)}")
     shape = x.shape
     tokens, hidden = shape
-    ldx = _pitch(x, "x")
+    ldx = _rows(x, shape, "x")
     kind, pres, ldres = native.IN_F32, None, 0
     if residual is not None:
         kind = IN_KINDS.get(residual.dtype)
         if kind is None or residual.shape != shape or residual.get_device() != index:
             raise ValueError(f"residual: expected {tuple(shape)} beside the first operand, got "
                              f"{residual.dtype} {tuple(residual.shape)} on {residual.device}")
-        pres, ldres = residual.data_ptr(), _pitch(residual, "residual")
+        pres, ldres = residual.data_ptr(), _rows(residual, shape, "residual")
     elif residual_out is not None:
         raise ValueError("residual_out without a residual")
     if next_weight is None and (residual is None or quantize or out_dtype is not None):
         raise ValueError("next_weight is missing: there is nothing to norm, quantise or return")
     if quantize and out_dtype is not None:
         raise ValueError("codes have no out_dtype")
+    if tokens > MAX_ROWS:
+        _too_many("x", tokens)
+    if hidden > MAX_HIDDEN:
+        raise ValueError(f"rows of {hidden}, at most {MAX_HIDDEN}")
     row = (hidden,)
     ppost = None if post_weight is None else _vector(post_weight, row, "post_weight", index)
     pnext = None if next_weight is None else _vector(next_weight, row, "next_weight", index)

@@ -64,6 +64,9 @@ class Int8Workload(Workload):
         self._check_supported()
         return self.call(inputs)
 
+    def check_status(self) -> None:
+        int8.check_status(self.device)
+
 
 @register(name="int8_gemm", supported_arches=("sm_100a",))
 class Int8GEMM(Int8Workload):

@@ -488,6 +488,7 @@ def test_workload_smoke_cases(name):
             workload.validate(workload.get_reference(inputs), out)
             launch, _ = workload.prepare(inputs)
             workload.validate(out, launch())
+        workload.check_status()
 
 
 def test_offsets_and_placement_of_pairs():
@@ -640,3 +641,39 @@ def test_block_around_the_fp4_layer():
     plain = norm_plain(y, residual, post, None, 1.0, pre, 1e-6)
     assert_norm((got, normed, None), torch.bfloat16, torch.bfloat16, plain)
     layer.close()
+
+
+def test_offsets_beyond_32_bits():
+    """Operands and results whose last elements lie more than 2^31 elements and 2^32 bytes in."""
+    g = rng_of(99)
+    m, n, k = 70001, 32768, 16
+    a, b = make_codes(g, m, k), make_codes(g, n, k)
+    sa, sb = torch.rand(m, device=DEV, generator=g), torch.rand(n, device=DEV, generator=g)
+    y = int8.gemm(a, b, sa, sb)
+    for rows in (slice(0, 3), slice(m - 3, m)):
+        assert_product(y[rows], a[rows], b, sa[rows], sb)
+    del y
+    experts, n, k = 20, 16384, 16384                  # 5.4 GB of weights
+    b = torch.empty((experts, n, k), dtype=torch.int8, device=DEV)
+    b.view(torch.int32).random_(generator=g)
+    a, sa = make_codes(g, 6, k), torch.rand(6, device=DEV, generator=g)
+    sb = torch.rand((experts, n), device=DEV, generator=g)
+    offsets = torch.zeros(experts + 1, dtype=torch.int32, device=DEV)
+    offsets[1:] = 2
+    offsets[experts] = 6
+    y = int8.grouped_gemm(a, b, sa, sb, offsets, out_dtype=torch.float32)
+    assert_product(y[:2], a[:2], b[0], sa[:2], sb[0])
+    assert_product(y[2:], a[2:], b[-1], sa[2:], sb[-1])
+    del b
+    tokens, hidden = 262147, 8200
+    x = torch.empty((tokens, hidden), dtype=torch.bfloat16, device=DEV)
+    x.normal_(generator=g)
+    q, s = int8.quantize_tokens(x)
+    assert_quantized((q[-3:], s[-3:]), x[-3:])
+    del q
+    w = 0.5 + torch.rand(hidden, device=DEV, generator=g)
+    out = int8.residual_norm(x, x, post_weight=w, next_weight=w)
+    last = tuple(t[-3:] if t is not None else None for t in out)
+    assert_norm(last, torch.bfloat16, torch.bfloat16, norm_plain(x[-3:], x[-3:], w, None, 1.0, w, 1e-6))
+    del out
+    torch.cuda.empty_cache()

@@ -44,6 +44,10 @@ def test_functions_refuse_what_they_cannot_take():
         lambda: int8.grouped_gemm(a, codes(2, 8, 32), sa, ones(2, 8), torch.zeros(3, dtype=torch.int64)),
         lambda: int8.grouped_gemm(a, codes(2, 8, 32), sa, ones(2, 8), torch.zeros(2, dtype=torch.int32)),
         lambda: int8.grouped_gemm(a, codes(2, 8, 32), sa, ones(16), torch.zeros(3, dtype=torch.int32)),
+        lambda: int8.gemm(codes(1, 16).expand((1 << 30) + 1, 16), b[:, :16], sa, sb),   # too many rows
+        lambda: int8.quantize_tokens(ones(1, 1).expand(1 << 32, 1)),
+        lambda: int8.residual_norm(ones(1, 1).expand(1 << 32, 1), next_weight=ones(1)),
+        lambda: int8.residual_norm(ones(1, 32769), next_weight=ones(32769)),
         lambda: int8.quantize_tokens(ones(4)),
         lambda: int8.quantize_tokens(ones(4, 4).double()),
         lambda: int8.quantize_tokens(ones(4, 4).T[:, ::2]),
@@ -79,6 +83,8 @@ def test_entry_points_refuse_before_cuda(library):
     assert gemm(ldd=4) == native.E_INVALID_ARGUMENT
     assert gemm(m=-1) == native.E_UNSUPPORTED_SHAPE
     assert gemm(n=0) == native.E_UNSUPPORTED_SHAPE
+    assert gemm(m=(1 << 30) + 1) == native.E_UNSUPPORTED_SHAPE
+    assert gemm(n=(1 << 30) + 1, ldd=1 << 31) == native.E_UNSUPPORTED_SHAPE
     assert gemm(k=0) == native.E_UNSUPPORTED_SHAPE
     assert gemm(k=131072, lda=131072, ldb=131072) == native.E_UNSUPPORTED_SHAPE
     assert gemm(a=24) == native.E_MISALIGNED
