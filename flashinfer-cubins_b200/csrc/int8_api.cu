@@ -191,7 +191,7 @@ int launch_product(const Product& q, void* stream) {
   if (int rc = check_product(q)) return rc;
   if (q.rows == 0) return 0;
   const int sms = host_sm_count();
-  Tiling tiling = choose_tiling(q, sms);
+  const Tiling tiling = choose_tiling(q, sms);
   const int ctas = tiling.ctas, tile_tokens = tiling.tile_tokens, split = tiling.split;
   const int channels = (q.gated ? 64 : 128) * ctas;
   const long long n_tiles = (q.n + channels - 1) / channels;
@@ -313,6 +313,7 @@ RowGrid row_grid(int rows, int width, int p, int elements) {
   g.elements = p == 8 && rows > 2 * host_sm_count() ? elements : 8;
   while ((width + g.elements - 1) / g.elements > 1024) g.elements *= 2;
   // One CTA of 1,024 threads on an SM is one row under way: two of 512 with twice the work.
+  if (p == 8 && rows > 2 * host_sm_count() && g.elements == 16 && width > 8192) g.elements = 32;
   g.threads = ((width + g.elements - 1) / g.elements + 31) / 32 * 32;
   if (p == 1) {  // the shapes that there are kernels for
     if (g.elements > 8) {
