@@ -62,8 +62,8 @@ struct Product {
 };
 
 int check_product(const Product& p) {
-  if (p.rows < 0 || p.rows > kMaxRows || p.n < 1 || p.n > (p.gated ? kMaxRows / 2 : kMaxRows) || p.k < 1 || p.k > kMaxDepth || p.experts < 1 ||
-      p.experts > kInt8MaxExperts) {
+  if (p.rows < 0 || p.rows > kMaxRows || p.n < 1 || p.n > (p.gated ? kMaxRows / 2 : kMaxRows) ||
+      p.k < 1 || p.k > kMaxDepth || p.experts < 1 || p.experts > kInt8MaxExperts) {
     return fail(NVFP4_E_UNSUPPORTED_SHAPE,
                 "unsupported product: %d rows, n=%d, k=%d (at most %d), %d experts (at most %d)",
                 p.rows, p.n, p.k, kMaxDepth, p.experts, kInt8MaxExperts);
@@ -94,9 +94,7 @@ int check_product(const Product& p) {
 using TileKernel = void (*)(Int8TileParams);
 
 TileKernel tile_kernel(int ctas, int sub, bool gated) {
-  if (ctas == 1) {
-    return gated ? int8_tile_kernel<1, 2, true> : int8_tile_kernel<1, 2, false>;
-  }
+  if (ctas == 1) return gated ? int8_tile_kernel<1, 2, true> : int8_tile_kernel<1, 2, false>;
   if (sub == 1) return gated ? int8_tile_kernel<2, 1, true> : int8_tile_kernel<2, 1, false>;
   return gated ? int8_tile_kernel<2, 2, true> : int8_tile_kernel<2, 2, false>;
 }
@@ -222,8 +220,15 @@ int launch_product(const Product& q, void* stream) {
   const cuuint64_t a_strides[1] = {static_cast<cuuint64_t>(q.lda)};
   const cuuint32_t a_box[2] = {128, static_cast<cuuint32_t>(tile_tokens / ctas)};
   if (int rc = encode(&p.map_a, q.a, 2, a_dims, a_strides, a_box)) return rc;
-  const cuuint32_t part_box[2] = {128, static_cast<cuuint32_t>(32 / ctas)};
-  if (int rc = encode(&p.map_a_part, q.a, 2, a_dims, a_strides, part_box)) return rc;
+  // Only a tile of fewer MMA columns than the others reads through the second map: the last one of a
+  // dense product, any group's last one of a grouped product (of one expert, too).
+  const int last = q.rows % tile_tokens;
+  if (q.offsets != nullptr || (last != 0 && (last + 31) / 32 * 32 != tile_tokens)) {
+    const cuuint32_t part_box[2] = {128, static_cast<cuuint32_t>(32 / ctas)};
+    if (int rc = encode(&p.map_a_part, q.a, 2, a_dims, a_strides, part_box)) return rc;
+  } else {
+    p.map_a_part = p.map_a;
+  }
   p.a_scales = q.a_scales;
   p.b_scales = q.b_scales;
   p.bias = q.bias;
@@ -246,8 +251,7 @@ int launch_product(const Product& q, void* stream) {
 
   const TileKernel kernel = tile_kernel(ctas, tiling.sub, q.gated);
   CUDA_TRY(cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                                cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                kSharedLimit));
+                                cudaFuncAttributeMaxDynamicSharedMemorySize, kSharedLimit));
   const int group = split > 1 ? split : ctas;
   // A split tile is a cluster's only one; otherwise a CTA (or pair) on every SM walks the tiles.
   const long long groups = split > 1 ? tiles : std::min<long long>(tiles, sms / ctas);

@@ -40,7 +40,9 @@ constexpr int int8_parts(int tile_tokens) {
 constexpr int int8_threads(int tile_tokens) { return 64 + 128 * int8_parts(tile_tokens); }
 constexpr int kInt8MaxStages = 12;
 constexpr int kInt8MaxExperts = 1024;
-constexpr int kInt8Band = 8;  // token tiles that are walked together, channel tile by channel tile
+// Token tiles that are walked together, channel tile by channel tile, for the L2 cache: 8192^3 takes 348,
+// 340 and 333 us with bands of 4, 8 and 16, 32 experts of 4096 rows, gated 2048 x 7168, 183, 184 and 187.
+constexpr int kInt8Band = 8;
 
 struct Int8TileParams {
   // Weights: [experts][1][n][k], box 128 rows of 128 bytes. Gated: [experts][n / 16][2][16][k], box

@@ -42,6 +42,7 @@ MAX_ROWS = 1 << 30  # rows of an operand; n at most half of that
 _INT8, _FLOAT = torch.int8, torch.float32
 _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
+_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
 _supported: dict[int, bool] = {}
 
 
@@ -57,7 +58,7 @@ def _check_device(index: int) -> None:
 def _launch(index: int, entry: str, *arguments) -> None:
     """Call a C entry point on device ``index`` and its current stream."""
     function = getattr(native.load(), entry)
-    if index == torch.cuda.current_device():
+    if index == _current_device():
         status = function(*arguments, _raw_stream(index))
     else:
         with torch.cuda.device(index):
@@ -66,10 +67,8 @@ def _launch(index: int, entry: str, *arguments) -> None:
         native.check(status)
 
 
-def _refuse_gradients(*tensors) -> None:
-    for t in tensors:
-        if t is not None and t.requires_grad:
-            raise ValueError("the INT8 operators have no backward; call them under torch.no_grad()")
+def _refuse_gradients() -> None:
+    raise ValueError("the INT8 operators have no backward; call them under torch.no_grad()")
 
 
 def check_status(device: torch.device | str | int | None = None) -> None:
@@ -139,8 +138,10 @@ def gemm(a: torch.Tensor, b: torch.Tensor, a_scales: torch.Tensor, b_scales: tor
     FP32). With ``gated`` ``b`` is ``[2n, k]``, gate rows before up rows, and the result
     ``silu(gate) * up`` ``[m, n]``. ``out``: a tensor to write it to."""
     index = a.get_device()
-    if torch.is_grad_enabled():
-        _refuse_gradients(a_scales, b_scales, bias, out)
+    if torch.is_grad_enabled() and (a_scales.requires_grad or b_scales.requires_grad
+                                    or (bias is not None and bias.requires_grad)
+                                    or (out is not None and out.requires_grad)):
+        _refuse_gradients()
     lda, ldb = _codes(a, 2, "a", index), _codes(b, 2, "b", index)
     (m, k), (width, depth) = a.shape, b.shape
     if depth != k:
@@ -173,8 +174,9 @@ def grouped_gemm(a: torch.Tensor, b: torch.Tensor, a_scales: torch.Tensor, b_sca
     never by the host. Rows that no expert owns are left as they were in ``out`` (and hold anything
     in a result made here)."""
     index = a.get_device()
-    if torch.is_grad_enabled():
-        _refuse_gradients(a_scales, b_scales, out)
+    if torch.is_grad_enabled() and (a_scales.requires_grad or b_scales.requires_grad
+                                    or (out is not None and out.requires_grad)):
+        _refuse_gradients()
     lda, ldb = _codes(a, 2, "a", index), _codes(b, 3, "b", index)
     (rows, k), (experts, width, depth) = a.shape, b.shape
     if depth != k:
@@ -211,8 +213,8 @@ def quantize_tokens(x: torch.Tensor, *, rows: torch.Tensor | None = None,
     ``[R]`` on the device) gathers: row r of the codes is row ``rows[r]`` of ``x``; an index outside
     ``[0, tokens)`` leaves row r as it was. ``out``: codes and scales to write to."""
     index = x.get_device()
-    if torch.is_grad_enabled():
-        _refuse_gradients(x)
+    if x.requires_grad and torch.is_grad_enabled():
+        _refuse_gradients()
     kind = IN_KINDS.get(x.dtype)
     if x.dim() != 2 or kind is None:
         raise ValueError(f"x: expected 2-d FP32, BF16 or FP16, got {x.dtype} {tuple(x.shape)}")
@@ -261,8 +263,9 @@ def residual_norm(x: torch.Tensor, residual: torch.Tensor | None = None, *,
     for ``tokens / gates`` consecutive tokens. Weights and gate are FP32. Without a residual only
     ``y = x / rms(x) * next_weight`` is made. ``residual_out`` may be ``residual`` itself."""
     index, device = x.get_device(), x.device
-    if torch.is_grad_enabled():
-        _refuse_gradients(x, residual, post_weight, gate, next_weight)
+    if torch.is_grad_enabled() and any(
+            t is not None and t.requires_grad for t in (x, residual, post_weight, gate, next_weight, residual_out)):
+        _refuse_gradients()
     x_kind = IN_KINDS.get(x.dtype)
     if x.dim() != 2 or x_kind is None:
         raise ValueError(f"x: expected 2-d FP32, BF16 or FP16, got {x.dtype} {tuple(x.shape)}")

@@ -164,6 +164,24 @@ def test_grouped_product(counts, n, k, gated):
                 assert_product(out[lo:hi], a[lo:hi], b[e], sa[lo:hi], sb[e], None, gated)
 
 
+@pytest.mark.parametrize("rows", [32, 64, 96, 128, 256, 512])
+def test_one_expert_that_owns_few_of_the_rows(rows):
+    """The tile is made for all rows of the buffers, the group has fewer: its MMA is narrower than
+    the tile's full copy."""
+    g = rng_of(rows)
+    a, b = make_codes(g, rows, 384), make_codes(g, 1, 200, 384)
+    sa, sb = torch.rand(rows, device=DEV, generator=g), torch.rand((1, 200), device=DEV, generator=g)
+    for lo, hi in ((0, 10), (3, rows // 2), (rows - 1, rows), (0, rows), (5, 5)):
+        out, check = guarded(rows, 200, torch.float32)
+        int8.grouped_gemm(a, b, sa, sb, torch.tensor([lo, hi], dtype=torch.int32, device=DEV),
+                          out_dtype=torch.float32, out=out)
+        check()
+        assert (out[:lo] == 77.0).all() and (out[hi:] == 77.0).all()
+        if hi > lo:
+            assert_product(out[lo:hi], a[lo:hi], b[0], sa[lo:hi], sb[0])
+    int8.check_status(DEV)
+
+
 def test_grouped_product_of_strided_experts_equals_the_dense_one():
     g = rng_of(9)
     b = make_codes(g, 6, 200, 96)[::2]
@@ -677,3 +695,45 @@ def test_offsets_beyond_32_bits():
     assert_norm(last, torch.bfloat16, torch.bfloat16, norm_plain(x[-3:], x[-3:], w, None, 1.0, w, 1e-6))
     del out
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("tokens", [9, 400])
+@pytest.mark.parametrize("k", [24, 25, 2048, 2050, 9000, 20008])
+def test_quantiser_finds_every_extreme(dtype, tokens, k):
+    """The largest magnitude at every kind of place and of either sign, infinities and NaN of either
+    sign, in the few-row and many-row kernels of every row length."""
+    g = rng_of(k + tokens)
+    x = torch.randn((tokens, k), device=DEV, generator=g).to(dtype)
+    at = torch.randint(0, k, (tokens,), device=DEV, generator=g)
+    at[0], at[1], at[2], at[3] = 0, k - 1, k - 2, k // 2
+    sign = torch.where(torch.arange(tokens, device=DEV) % 2 == 0, 1.0, -1.0)
+    x[torch.arange(tokens, device=DEV), at] = (sign * 57.0).to(dtype)
+    x[5] = -x[5].abs()
+    x[6] = x[6].abs()
+    assert_quantized(int8.quantize_tokens(x), x)
+    for value in (float("inf"), float("-inf"), float("nan"), -float("nan")):
+        y = x.clone()
+        y[torch.arange(tokens, device=DEV), at] = value
+        q, s = int8.quantize_tokens(y)
+        assert not q.any() and not torch.isfinite(s).any()
+        assert torch.isnan(s).all() if value != value else (s == float("inf")).all()
+        _, q, s = int8.residual_norm(y, next_weight=torch.ones(k, device=DEV), quantize=True)
+        assert not q.any() and torch.isnan(s).all()
+
+
+def test_norm_codes_do_not_depend_on_how_rows_lie():
+    """The same rows a few at a time and many at once, in whole pieces and one element at a time:
+    the same codes and scales, bit for bit (the statistic is taken in 64 bits)."""
+    g = rng_of(123)
+    for hidden in (640, 4096, 8192, 16384):
+        x = torch.randn((600, hidden), device=DEV, generator=g).bfloat16()
+        residual = torch.randn((600, hidden), device=DEV, generator=g).half()
+        w = 0.5 + torch.rand(hidden, device=DEV, generator=g)
+        many = int8.residual_norm(x, residual, post_weight=w, next_weight=w, quantize=True)
+        few = int8.residual_norm(x[:3], residual[:3], post_weight=w, next_weight=w, quantize=True)
+        shifted = torch.empty((600, hidden + 1), dtype=x.dtype, device=DEV)
+        shifted[:, 1:] = x
+        single = int8.residual_norm(shifted[:, 1:], residual, post_weight=w, next_weight=w, quantize=True)
+        for a, b, c in zip(many, few, single):
+            assert torch.equal(a[:3], b) and torch.equal(a, c)
