@@ -248,6 +248,11 @@ int8_tile_kernel(const __grid_constant__ Int8TileParams p) {
     abort_flag = 0;
     mbar_fence_init();
   }
+  if (warp == 0 && lane == 0) {  // the maps are launch parameters: nothing to wait for
+    prefetch_tensormap(&p.map_b);
+    prefetch_tensormap(&p.map_a);
+    prefetch_tensormap(&p.map_a_part);
+  }
   if (warp == 1) {
     if constexpr (CTAS == 1) {
       tmem_alloc(smem_u32(&tmem_base_slot), tmem_cols);
@@ -262,11 +267,6 @@ int8_tile_kernel(const __grid_constant__ Int8TileParams p) {
   grid_dependency_wait();
   grid_launch_dependents();
   if (warp == 0) {
-    if (lane == 0) {
-      prefetch_tensormap(&p.map_b);
-      prefetch_tensormap(&p.map_a);
-      prefetch_tensormap(&p.map_a_part);
-    }
     // First rows: the offsets cut to [0, rows], and where they decrease their running maximum, so
     // that no value of theirs makes groups overlap or reach outside. Then a prefix over the
     // experts' token tiles.
@@ -340,6 +340,17 @@ int8_tile_kernel(const __grid_constant__ Int8TileParams p) {
     return tile;
   };
 
+  // Where a tile begins in k (it goes round): a single CTA's channel tiles begin in different places, so
+  // that the SMs do not all read the same columns of rows a power of two apart (one token: 8192 x 8192
+  // 16.1 us from the start of k, 15.0 so; 16384 x 8192 25.3 and 23.4). Pairs work on more tokens and are
+  // not bound by memory; the loops are shorter without it.
+  constexpr bool kRound = CTAS == 1;
+  auto first_piece = [&](const Int8Tile& tile) {
+    if constexpr (!kRound) return kt0;
+    const uint32_t steps = static_cast<uint32_t>(kt1 - kt0 + SUB - 1) / SUB;
+    return kt0 + static_cast<int>(static_cast<uint32_t>(tile.n_tile) * 5u % steps) * SUB;
+  };
+
   if (warp == 0) {
     // ------------------------------------------------------------------ producer
     // One thread runs the whole loop, here and in the MMA warp: electing it anew at every step cost
@@ -358,8 +369,8 @@ int8_tile_kernel(const __grid_constant__ Int8TileParams p) {
         const int share = tile.columns / CTAS;  // tokens this CTA loads
         const int token0 = tile.m0 + static_cast<int>(CTAS == 2 ? rank : 0) * share;
         const uint32_t bytes = CTAS * (weight_bytes + static_cast<uint32_t>(share) * 128u);
-        int k = kt0 * 128;
-        for (int kt = kt0; kt < kt1; kt += SUB) {
+        int kt = first_piece(tile);
+        for (int i0 = kt0; i0 < kt1; i0 += SUB) {
           if (!mbar_wait(empty0 + 8 * stage, phase, abort_ptr)) {
             int8_give_up(abort_ptr, kInt8ProducerTimeout);
             ok = false;
@@ -377,6 +388,7 @@ int8_tile_kernel(const __grid_constant__ Int8TileParams p) {
 #pragma unroll
           for (int i = 0; i < SUB; ++i) {
             if (i >= parts) break;
+            const int k = (kt + i) * 128;
             if (GATED && p.whole) {
               tma_gated_weights<CTAS>(w, &p.map_b, bar, k, channel0 / 16, tile.expert);
             } else if constexpr (GATED) {
@@ -394,10 +406,11 @@ int8_tile_kernel(const __grid_constant__ Int8TileParams p) {
                 tma_rows<CTAS>(r + c * 128, &p.map_a_part, bar, k, token0 + c);
               }
             }
-            k += 128;
             w += weight_bytes;
             r += token_bytes;
           }
+          kt += SUB;
+          if (kRound && kt >= kt1) kt = kt0;
           w_dst = stage == 0 ? smem_base : w_dst + stage_bytes;
         }
       }
@@ -429,10 +442,8 @@ int8_tile_kernel(const __grid_constant__ Int8TileParams p) {
         tc_fence_after_sync();
         const uint32_t d = tmem_base + acc * tile_tokens;
         uint32_t accumulate = 0;
-        // k of this and the later stages. The last one's k beyond the depth is zero in both operands
-        // and not multiplied.
-        int left = min(p.k, kt1 * 128) - kt0 * 128;
-        for (int kt = kt0; kt < kt1; kt += SUB) {
+        int kt = first_piece(tile);
+        for (int i0 = kt0; i0 < kt1; i0 += SUB) {
           if (!mbar_wait(full0 + 8 * stage, phase, abort_ptr)) {
             int8_give_up(abort_ptr, kInt8MmaInputTimeout);
             ok = false;
@@ -447,6 +458,8 @@ int8_tile_kernel(const __grid_constant__ Int8TileParams p) {
           uint32_t w = lo_w, r = lo_w + SUB * (weight_bytes >> 4);
 #pragma unroll
           for (int i = 0; i < SUB; ++i) {
+            // k of the last piece beyond the depth is zero in both operands and not multiplied.
+            const int left = min(p.k, kt1 * 128) - (kt + i) * 128;
             if (left > 96) {
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
@@ -460,10 +473,11 @@ int8_tile_kernel(const __grid_constant__ Int8TileParams p) {
               }
             }
             accumulate = 1;
-            left -= 128;
             w += weight_bytes >> 4;
             r += token_bytes >> 4;
           }
+          kt += SUB;
+          if (kRound && kt >= kt1) kt = kt0;
           int8_commit<CTAS>(empty);
           lo_w = stage == 0 ? lo0 : lo_w + (stage_bytes >> 4);
         }
