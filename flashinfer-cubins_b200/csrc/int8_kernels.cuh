@@ -602,7 +602,8 @@ __global__ void __launch_bounds__(1024) int8_quantize_long_kernel(const Quantize
 // ---------------------------------------------------------------------------
 
 // x * sigmoid(x) with the approximate exponential and reciprocal (2^-22 and 2^-23 relative): no slow
-// path where exp(-x) overflows, its reciprocal is 0 there.
+// path where exp(-x) overflows, its reciprocal is 0 there (from x = -87.3 on, where the value is
+// below 1e-36).
 __device__ __forceinline__ float silu(float x) {
   float e, r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x * -1.4426950408889634f));

@@ -248,7 +248,8 @@ def residual_norm(x: torch.Tensor, residual: torch.Tensor | None = None, *,
                   post_weight: torch.Tensor | None = None, gate: torch.Tensor | None = None,
                   residual_scale: float = 1.0, next_weight: torch.Tensor | None = None,
                   eps: float = 1e-6, quantize: bool = False, out_dtype: torch.dtype | None = None,
-                  residual_out: torch.Tensor | None = None
+                  residual_out: torch.Tensor | None = None,
+                  out: torch.Tensor | tuple[torch.Tensor, torch.Tensor] | None = None
                   ) -> tuple[torch.Tensor | None, torch.Tensor | None, torch.Tensor | None]:
     """The end of one block and the start of the next, for ``x [tokens, hidden]``, the block's
     output, and the ``residual`` stream (any of FP32, BF16, FP16 each)::
@@ -261,7 +262,8 @@ def residual_norm(x: torch.Tensor, residual: torch.Tensor | None = None, *,
     ``out_dtype`` (default: the residual's type) or, with ``quantize``, as INT8 codes with their
     ``scales``; what is not made is None. ``gate`` is ``[hidden]`` or ``[gates, hidden]``, each row
     for ``tokens / gates`` consecutive tokens. Weights and gate are FP32. Without a residual only
-    ``y = x / rms(x) * next_weight`` is made. ``residual_out`` may be ``residual`` itself."""
+    ``y = x / rms(x) * next_weight`` is made. ``residual_out`` (may be ``residual`` itself) and ``out``
+    (``y``, or codes and scales) are tensors to write to."""
     index, device = x.get_device(), x.device
     if torch.is_grad_enabled() and any(
             t is not None and t.requires_grad for t in (x, residual, post_weight, gate, next_weight, residual_out)):
@@ -285,6 +287,8 @@ def residual_norm(x: torch.Tensor, residual: torch.Tensor | None = None, *,
         raise ValueError("next_weight is missing: there is nothing to norm, quantise or return")
     if quantize and out_dtype is not None:
         raise ValueError("codes have no out_dtype")
+    if out is not None and next_weight is None:
+        raise ValueError("out without next_weight")
     if tokens > MAX_ROWS:
         _too_many("x", tokens)
     if hidden > MAX_HIDDEN:
@@ -307,15 +311,23 @@ def residual_norm(x: torch.Tensor, residual: torch.Tensor | None = None, *,
     y, py, ldy, y_kind, scales, pscales = None, None, 0, native.NORM_CODES, None, None
     if next_weight is not None:
         if quantize:
-            y, ldy = empty_codes(tokens, hidden, device), -(-hidden // 16) * 16
-            scales = torch.empty(tokens, dtype=torch.float32, device=device)
-            pscales = scales.data_ptr()
+            if out is None:
+                y, ldy = empty_codes(tokens, hidden, device), -(-hidden // 16) * 16
+                scales = torch.empty(tokens, dtype=torch.float32, device=device)
+                pscales = scales.data_ptr()
+            else:
+                y, scales = out
+                ldy = _given(y, shape, torch.int8, index, "out")
+                pscales = _vector(scales, (tokens,), "out", index)
         else:
             dtype = out_dtype or (x if residual is None else residual).dtype
             y_kind = IN_KINDS.get(dtype)
             if y_kind is None:
                 raise ValueError(f"no output in {dtype}")
-            y, ldy = torch.empty(tokens, hidden, dtype=dtype, device=device), hidden
+            if out is None:
+                y, ldy = torch.empty(tokens, hidden, dtype=dtype, device=device), hidden
+            else:
+                y, ldy = out, _given(out, shape, dtype, index, "out")
         py = y.data_ptr()
     _launch(index, "nvfp4_residual_norm", x.data_ptr(), x_kind, ldx, pres, kind, ldres, ppost, pgate, gates,
             residual_scale, pnext, eps, pr, ldr, py, y_kind, ldy, pscales, tokens, hidden)

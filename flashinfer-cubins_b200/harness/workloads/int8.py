@@ -54,15 +54,26 @@ def rms_normed(x: torch.Tensor, weight: torch.Tensor, eps: float) -> torch.Tenso
 
 class Int8Workload(Workload):
     """``run`` calls the function of ``harness.int8`` on the workload's device; nothing is kept
-    between calls, so there is no plan or workspace to prepare."""
+    between calls, so there is no plan or workspace to prepare, only the outputs."""
 
-    def call(self, inputs: tuple) -> tuple:
+    def call(self, inputs: tuple, outputs: tuple | None = None) -> tuple:
+        """The outputs of ``inputs``, new ones or those given."""
         raise NotImplementedError
 
     def run(self, inputs):
         self._check_open()
         self._check_supported()
         return self.call(inputs)
+
+    def prepare(self, inputs):
+        outputs = self.run(inputs)
+
+        def launch() -> tuple:
+            self._check_open()
+            self.call(inputs, outputs)
+            return outputs
+
+        return launch, outputs
 
     def check_status(self) -> None:
         int8.check_status(self.device)
@@ -110,9 +121,10 @@ class Int8GEMM(Int8Workload):
     def get_reference(self, inputs):
         return (scaled_product(*inputs),)
 
-    def call(self, inputs):
-        a, b, sa, sb, bias, gated, out = inputs
-        return (int8.gemm(a, b, sa, sb, bias=bias, gated=gated, out_dtype=out),)
+    def call(self, inputs, outputs=None):
+        a, b, sa, sb, bias, gated, dtype = inputs
+        return (int8.gemm(a, b, sa, sb, bias=bias, gated=gated, out_dtype=dtype,
+                          out=outputs and outputs[0]),)
 
     def validate(self, ref, impl):
         # The same exact sums; a rounding of the output type, and in the gate FP32 ones.
@@ -165,9 +177,10 @@ class Int8GroupGEMM(Int8Workload):
             scaled_product(a[lo:hi], b[e], sa[lo:hi], sb[e], None, gated, dtype)
             for e, (lo, hi) in enumerate(zip(edges, edges[1:]))]),)
 
-    def call(self, inputs):
-        a, b, sa, sb, offsets, gated, out = inputs
-        return (int8.grouped_gemm(a, b, sa, sb, offsets, gated=gated, out_dtype=out),)
+    def call(self, inputs, outputs=None):
+        a, b, sa, sb, offsets, gated, dtype = inputs
+        return (int8.grouped_gemm(a, b, sa, sb, offsets, gated=gated, out_dtype=dtype,
+                                  out=outputs and outputs[0]),)
 
     validate = Int8GEMM.validate
 
@@ -197,8 +210,8 @@ class Int8Quantize(Int8Workload):
         x, rows = inputs
         return quantized(x if rows is None else x[rows.long()])
 
-    def call(self, inputs):
-        return int8.quantize_tokens(inputs[0], rows=inputs[1])
+    def call(self, inputs, outputs=None):
+        return int8.quantize_tokens(inputs[0], rows=inputs[1], out=outputs)
 
     def validate(self, ref, impl):
         # Both quotients are correctly rounded: the same codes and scales, bit for bit.
@@ -241,11 +254,12 @@ class ResidualNorm(Int8Workload):
         y = rms_normed(r, weight, eps)
         return (r.to(residual.dtype), *quantized(y)) if codes else (r.to(residual.dtype), y.to(residual.dtype))
 
-    def call(self, inputs):
+    def call(self, inputs, outputs=None):
         x, residual, post, gate, scale, weight, eps, codes = inputs
-        outputs = int8.residual_norm(x, residual, post_weight=post, gate=gate, residual_scale=scale,
-                                     next_weight=weight, eps=eps, quantize=codes)
-        return tuple(t for t in outputs if t is not None)
+        r, y = (None, None) if outputs is None else (outputs[0], outputs[1:] if codes else outputs[1])
+        made = int8.residual_norm(x, residual, post_weight=post, gate=gate, residual_scale=scale,
+                                  next_weight=weight, eps=eps, quantize=codes, residual_out=r, out=y)
+        return tuple(t for t in made if t is not None)
 
     def validate(self, ref, impl):
         # The kernel keeps the reference's order of roundings: the same bits, codes included.

@@ -387,6 +387,28 @@ def test_norm_over_sizes(tokens, hidden, kind):
     assert (off[:, 0] == 0).all() and (off[:, hidden + 1:] == 0).all()
 
 
+def test_norm_into_given_tensors():
+    g = rng_of(8)
+    x, residual = (torch.randn((37, 264), device=DEV, generator=g).bfloat16() for _ in range(2))
+    w = 0.5 + torch.rand(264, device=DEV, generator=g)
+    want = int8.residual_norm(x, residual, post_weight=w, next_weight=w, out_dtype=torch.float16)
+    view, check = guarded(37, 264, torch.float16)
+    r = torch.empty_like(residual)
+    got = int8.residual_norm(x, residual, post_weight=w, next_weight=w, out_dtype=torch.float16, out=view,
+                             residual_out=r)
+    assert got[0] is r and got[1] is view and torch.equal(r, want[0]) and torch.equal(view, want[1])
+    check()
+    want = int8.residual_norm(x, residual, post_weight=w, next_weight=w, quantize=True)
+    q, s = torch.empty((37, 300), dtype=torch.int8, device=DEV)[:, :264], torch.empty(37, device=DEV)
+    got = int8.residual_norm(x, residual, post_weight=w, next_weight=w, quantize=True, out=(q, s))
+    assert got[1] is q and torch.equal(q, want[1]) and torch.equal(s, want[2])
+    for bad in (torch.empty((37, 264), device=DEV), torch.empty((36, 264), dtype=torch.bfloat16, device=DEV)):
+        with pytest.raises(ValueError):
+            int8.residual_norm(x, residual, next_weight=w, out=bad)
+    with pytest.raises(ValueError):
+        int8.residual_norm(x, residual, out=view)
+
+
 def test_norm_of_special_rows():
     """Zero rows give zeros, infinite and NaN rows poison only themselves."""
     x = torch.ones((5, 300), device=DEV)
@@ -504,8 +526,11 @@ def test_workload_smoke_cases(name):
             inputs = workload.get_inputs(case)
             out = workload.run(inputs)
             workload.validate(workload.get_reference(inputs), out)
-            launch, _ = workload.prepare(inputs)
-            workload.validate(out, launch())
+            launch, outputs = workload.prepare(inputs)
+            allocated = torch.cuda.memory_stats()["allocation.all.allocated"]
+            assert launch() is outputs
+            assert torch.cuda.memory_stats()["allocation.all.allocated"] == allocated
+            workload.validate(out, outputs)
         workload.check_status()
 
 
