@@ -86,9 +86,10 @@ def _too_many(what: str, count: int) -> None:
 
 def _rows(t: torch.Tensor, shape, what: str) -> int:
     """Elements between the rows of ``t`` (its last but one dimension; ``shape`` is its shape)."""
-    if shape[-1] > 1 and t.stride(-1) != 1:
+    stride = t.stride()
+    if stride[-1] != 1 and shape[-1] > 1:
         raise ValueError(f"{what}: elements of a row must be neighbours")
-    return t.stride(-2) if shape[-2] > 1 else -(-shape[-1] // 16) * 16  # one row: nothing lies between
+    return stride[-2] if shape[-2] > 1 else -(-shape[-1] // 16) * 16  # one row: nothing lies between
 
 
 def _vector(t: torch.Tensor, shape: tuple, what: str, index: int) -> int:
@@ -111,9 +112,10 @@ def _codes(t: torch.Tensor, dims: int, what: str, index: int) -> int:
     if t.dtype is not _INT8 or len(shape) != dims or t.get_device() != index:
         raise ValueError(f"{what}: expected {dims}-d int8 beside the first operand, got {t.dtype} "
                          f"{tuple(shape)} on {t.device}")
-    if shape[-1] > 1 and t.stride(-1) != 1:
+    stride = t.stride()
+    if stride[-1] != 1 and shape[-1] > 1:
         raise ValueError(f"{what}: elements of a row must be neighbours")
-    return t.stride(-2) if shape[-2] > 1 else -(-shape[-1] // 16) * 16
+    return stride[-2] if shape[-2] > 1 else -(-shape[-1] // 16) * 16
 
 
 def _given(out: torch.Tensor, shape: tuple, dtype: torch.dtype, index: int, what: str) -> int:
@@ -265,8 +267,11 @@ def residual_norm(x: torch.Tensor, residual: torch.Tensor | None = None, *,
     ``y = x / rms(x) * next_weight`` is made. ``residual_out`` (may be ``residual`` itself) and ``out``
     (``y``, or codes and scales) are tensors to write to."""
     index, device = x.get_device(), x.device
-    if torch.is_grad_enabled() and any(
-            t is not None and t.requires_grad for t in (x, residual, post_weight, gate, next_weight, residual_out)):
+    if torch.is_grad_enabled() and (
+            x.requires_grad or (residual is not None and residual.requires_grad)
+            or (post_weight is not None and post_weight.requires_grad) or (gate is not None and gate.requires_grad)
+            or (next_weight is not None and next_weight.requires_grad)
+            or (residual_out is not None and residual_out.requires_grad)):
         _refuse_gradients()
     x_kind = IN_KINDS.get(x.dtype)
     if x.dim() != 2 or x_kind is None:
