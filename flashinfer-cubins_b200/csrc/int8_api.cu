@@ -103,15 +103,18 @@ TileKernel tile_kernel(int ctas, int sub, bool gated) {
 // scales, 4.4 KB) and the slack that aligns the stages to 1,024 bytes.
 constexpr int kSharedLimit = 232448 - 5 * 1024;
 
+// Codes (128-byte swizzle), or with `output` 16-bit elements as they lie.
 int encode(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims,
-           const cuuint64_t* strides, const cuuint32_t* box) {
+           const cuuint64_t* strides, const cuuint32_t* box, bool output = false) {
   EncodeTiled encoder = nullptr;
   if (int rc = host_encoder(&encoder)) return rc;
   const cuuint32_t ones[5] = {1, 1, 1, 1, 1};
-  const CUresult res = encoder(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, rank, const_cast<void*>(base), dims,
-                               strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  const CUresult res = encoder(
+      map, output ? CU_TENSOR_MAP_DATA_TYPE_UINT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, rank,
+      const_cast<void*>(base), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+      output ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B,
+      output ? CU_TENSOR_MAP_L2_PROMOTION_NONE : CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (res != CUDA_SUCCESS) {
     return fail(static_cast<int>(res), "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(res));
   }
@@ -197,6 +200,9 @@ int launch_product(const Product& q, void* stream) {
   const long long m_tiles = q.experts == 1 ? (q.rows + tile_tokens - 1) / tile_tokens
                                            : q.rows / tile_tokens + std::min(q.experts, q.rows);
   const long long tiles = m_tiles * n_tiles;
+  if (tiles > (1ll << 31) - 1 - 1024) {  // and with a step of the walk behind them
+    return fail(NVFP4_E_UNSUPPORTED_SHAPE, "too many tiles: %d rows, n=%d, %d experts", q.rows, q.n, q.experts);
+  }
 
   Int8TileParams p{};
   const cuuint64_t half = static_cast<cuuint64_t>(q.n) * q.ldb;
@@ -229,6 +235,20 @@ int launch_product(const Product& q, void* stream) {
   } else {
     p.map_a_part = p.map_a;
   }
+  // 16-bit results leave through shared memory where the MMAs do not hide a store of 64 bytes a warp and
+  // CTAs take several tiles: 8192 x 8192 x 64 takes 41.4 us against 49.3 with direct stores, k = 256 35
+  // against 39.5, gated 4096 x 8192 x 256 55.4 against 58.5; k = 1024 57 against 58; k = 2048 95.0
+  // against 93.6. A CTA's only tile gains nothing: 300 x 4096 x 256 5.2 us against 5.0. The copies
+  // write 16 bytes at a time, so rows of D must start, follow and end on multiples of eight.
+  const long long walkers = sms / ctas;
+  p.staged = q.out_kind != NVFP4_OUT_F32 && q.k <= 1024 && split == 1 && tiles > walkers && q.n % 8 == 0 &&
+             q.ldd % 8 == 0 && aligned(q.d, 16);
+  if (p.staged) {
+    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(q.n), static_cast<cuuint64_t>(q.rows)};
+    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(q.ldd) * 2};
+    const cuuint32_t box[2] = {q.gated ? 16u : 32u, 32};
+    if (int rc = encode(&p.map_d, q.d, 2, dims, strides, box, true)) return rc;
+  }
   p.a_scales = q.a_scales;
   p.b_scales = q.b_scales;
   p.bias = q.bias;
@@ -245,7 +265,8 @@ int launch_product(const Product& q, void* stream) {
   p.tmem_columns = 32;
   while (p.tmem_columns < (split > 1 ? 1 : 2) * tile_tokens) p.tmem_columns *= 2;
   const int stage_bytes = tiling.sub * 128 * (128 + tile_tokens / ctas);
-  const int tables = 8 * (q.experts + 1);
+  const int tables = 8 * (q.experts + 1) +
+                     (p.staged ? 4 * int8_parts(tile_tokens) * static_cast<int>(kInt8StagedBytes) : 0);
   p.stages = std::min(kInt8MaxStages, (kSharedLimit - 1024 - tables) / stage_bytes);
   const size_t shared = static_cast<size_t>(p.stages) * stage_bytes + 1024 + tables;
 
@@ -254,7 +275,7 @@ int launch_product(const Product& q, void* stream) {
                                 cudaFuncAttributeMaxDynamicSharedMemorySize, kSharedLimit));
   const int group = split > 1 ? split : ctas;
   // A split tile is a cluster's only one; otherwise a CTA (or pair) on every SM walks the tiles.
-  const long long groups = split > 1 ? tiles : std::min<long long>(tiles, sms / ctas);
+  const long long groups = split > 1 ? tiles : std::min(tiles, walkers);
   cudaLaunchAttribute attribute[2];
   attribute[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attribute[0].val.programmaticStreamSerializationAllowed = 1;

@@ -6,7 +6,8 @@
 // (rows of A) its columns. A few tokens then cost a narrow MMA instead of an empty tile, the
 // weights stream through the wide operand, and in the epilogue a warp holds 32 neighbouring
 // channels of one token at a time, which are neighbours in D: every store instruction of a warp
-// is one run of 64 or 128 bytes, for any n, ldd and alignment, with no staging.
+// is one run of 64 or 128 bytes, for any n, ldd and alignment. Products of a small depth, whose time
+// is that of their results, stage 32 tokens of a warp's channels and store them by one copy.
 //
 // Warps of a CTA: 0 loads (one thread issues cp.async.bulk.tensor into a ring of
 // stages of 128 k), 1 issues tcgen05.mma.kind::i8 (32 k each) into one of two accumulators in
@@ -50,6 +51,7 @@ struct Int8TileParams {
   CUtensorMap map_b;
   CUtensorMap map_a;       // [rows][k], box of a whole tile's tokens (a pair: of half of them)
   CUtensorMap map_a_part;  // the same with a box of 32 (a pair: 16) rows
+  CUtensorMap map_d;       // staged: 16-bit [rows][n], box 32 rows of a warp's 32 (gated: 16) channels
   const float* a_scales;
   const float* b_scales;
   const float* bias;
@@ -62,7 +64,8 @@ struct Int8TileParams {
   int tmem_columns;
   int stages;
   int split;
-  int whole;  // gated: one copy brings a stage's weights
+  int whole;   // gated: one copy brings a stage's weights
+  int staged;  // D leaves through shared memory
 };
 
 // Set to a role's code when it abandons a wait; read and cleared by nvfp4_int8_status.
@@ -180,6 +183,30 @@ __device__ __forceinline__ int ld_cluster_s32(uint32_t addr) {
   return v;
 }
 
+// Stores a box from shared memory as part of the thread's current bulk group; what lies beyond the
+// tensor is not written.
+__device__ __forceinline__ void tma_store_rows(const void* map, uint32_t src, int channel, int row) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(src), "r"(channel), "r"(row)
+               : "memory");
+}
+
+// 32 tokens of a warp's channels through its 2 KB of shared memory, a 16-bit value at a time: the
+// addresses are constants apart, where a store to D needs one of its own.
+constexpr uint32_t kInt8StagedBytes = 2048;
+
+template <typename T, int COLUMNS>
+__device__ __forceinline__ void stage_columns(uint32_t to, uint32_t step, const float (&v)[COLUMNS]) {
+#pragma unroll
+  for (int i = 0; i < COLUMNS; ++i) {
+    const T value = from_float<T>(v[i]);
+    asm volatile("st.shared.b16 [%0], %1;" ::"r"(to + i * step),
+                 "h"(*reinterpret_cast<const unsigned short*>(&value))
+                 : "memory");
+  }
+}
+
 struct Int8Tile {
   int expert;
   int m0;      // first token (row of A)
@@ -231,8 +258,11 @@ int8_tile_kernel(const __grid_constant__ Int8TileParams p) {
   constexpr uint32_t weight_bytes = 128u * 128u;  // of a piece of 128 k
   const uint32_t token_bytes = static_cast<uint32_t>(tile_tokens / CTAS) * 128u;
   const uint32_t stage_bytes = SUB * (weight_bytes + token_bytes);
-  // Behind the stages: for every expert the token tiles of those before it, and its first row.
-  int* tiles_before = reinterpret_cast<int*>(dyn_smem + (smem_base - smem_u32(dyn_smem)) + stages * stage_bytes);
+  // Behind the stages: the epilogue warps' staging, if any; for every expert the token tiles of those
+  // before it, and its first row.
+  const uint32_t staging = smem_base + stages * stage_bytes;
+  int* tiles_before = reinterpret_cast<int*>(dyn_smem + (staging - smem_u32(dyn_smem)) +
+                                             (p.staged ? 4 * parts * kInt8StagedBytes : 0u));
   int* first_row = tiles_before + p.experts + 1;
   const uint32_t tmem_cols = p.tmem_columns;
 
@@ -309,24 +339,27 @@ int8_tile_kernel(const __grid_constant__ Int8TileParams p) {
 
   const int m_tiles = tiles_before[p.experts];
   const int n_tiles = (p.n + channels * CTAS - 1) / (channels * CTAS);
-  const long long tiles = static_cast<long long>(m_tiles) * n_tiles;
+  // 32 bits hold every tile's number (the host checks): the divisions below are done by every warp for
+  // every tile, and with 64-bit ones 8192 x 8192 x 64 takes 42.3 us for 41.4.
+  const uint32_t tiles = static_cast<uint32_t>(m_tiles) * static_cast<uint32_t>(n_tiles);
   const int group = p.split > 1 ? p.split : CTAS;  // CTAs that share a tile
-  const long long first_tile = blockIdx.x / group;
-  const long long step = gridDim.x / group;
+  const uint32_t first_tile = blockIdx.x / group;
+  const uint32_t step = gridDim.x / group;
   const int k_tiles = (p.k + 127) / 128;
   const int kt0 = p.split > 1 ? static_cast<int>(rank) * k_tiles / p.split : 0;
   const int kt1 = p.split > 1 ? (static_cast<int>(rank) + 1) * k_tiles / p.split : k_tiles;
 
   bool partials_written = false;  // a split tile's epilogue has passed the cluster's first barrier
 
-  auto decode = [&](long long t) {
+  auto decode = [&](uint32_t t) {
     Int8Tile tile;
-    const long long band_tiles = static_cast<long long>(kInt8Band) * n_tiles;
-    const int band = static_cast<int>(t / band_tiles);
-    const int in_band = static_cast<int>(t - band * band_tiles);
-    const int height = min(kInt8Band, m_tiles - band * kInt8Band);
-    const int m_tile = band * kInt8Band + in_band % height;
-    tile.n_tile = in_band / height;
+    const uint32_t band_tiles = kInt8Band * static_cast<uint32_t>(n_tiles);
+    const uint32_t band = t / band_tiles;
+    const uint32_t in_band = t - band * band_tiles;
+    const uint32_t height = min(kInt8Band, m_tiles - static_cast<int>(band) * kInt8Band);
+    const uint32_t across = in_band / height;
+    const int m_tile = static_cast<int>(band * kInt8Band + in_band - across * height);
+    tile.n_tile = static_cast<int>(across);
     // The last expert whose first tile is not behind m_tile, and that has tiles.
     int lo = 0, hi = p.experts;
     while (hi - lo > 1) {
@@ -363,7 +396,7 @@ int8_tile_kernel(const __grid_constant__ Int8TileParams p) {
       uint32_t phase = 1;
       uint32_t w_dst = smem_base;
       bool ok = true;
-      for (long long t = first_tile; ok && t < tiles; t += step) {
+      for (uint32_t t = first_tile; ok && t < tiles; t += step) {
         const Int8Tile tile = decode(t);
         const int channel0 = (tile.n_tile * CTAS + static_cast<int>(CTAS == 2 ? rank : 0)) * channels;
         const int share = tile.columns / CTAS;  // tokens this CTA loads
@@ -432,7 +465,7 @@ int8_tile_kernel(const __grid_constant__ Int8TileParams p) {
       uint32_t acc = 0, acc_phase = 1;
       uint32_t lo_w = lo0;
       bool ok = true;
-      for (long long t = first_tile; ok && t < tiles; t += step) {
+      for (uint32_t t = first_tile; ok && t < tiles; t += step) {
         const Int8Tile tile = decode(t);
         const uint32_t idesc = i8_instr_desc(128 * CTAS, static_cast<uint32_t>(tile.columns));
         if (!mbar_wait(smem_u32(&bar_acc_empty[acc]), acc_phase, abort_ptr)) {
@@ -495,25 +528,47 @@ int8_tile_kernel(const __grid_constant__ Int8TileParams p) {
     float* sa_stage = scale_stage[warp - 2];
     const uint32_t leader_acc_empty0 = CTAS == 1 ? smem_u32(&bar_acc_empty[0])
                                                  : cluster_map_shared(smem_u32(&bar_acc_empty[0]), 0);
-    uint32_t acc = 0, acc_phase = 0;
-    for (long long t = first_tile; t < tiles; t += step) {
-      const Int8Tile tile = decode(t);
-      // This lane's row of B: its channel in D, and its place among the scales.
-      const int channel0 = (tile.n_tile * CTAS + static_cast<int>(CTAS == 2 ? rank : 0)) * channels;
-      const int channel = GATED ? channel0 + quarter * 16 + (lane & 15) : channel0 + quarter * 32 + lane;
-      const bool live = channel < p.n;
+    // A tile as this lane sees it: its row of B is a channel of D and has a scale and a bias; its
+    // tokens are all of the tile's, or with a split this CTA's share, and the warp's two chunks of them
+    // have a scale each lane.
+    struct Share {
+      Int8Tile tile;
+      int channel, c_begin, c_end;
+      float sb, bias, sa[2];
+    };
+    auto share_of = [&](uint32_t t) {
+      Share s;
+      s.tile = decode(t);
+      const int channel0 = (s.tile.n_tile * CTAS + static_cast<int>(CTAS == 2 ? rank : 0)) * channels;
+      s.channel = GATED ? channel0 + quarter * 16 + (lane & 15) : channel0 + quarter * 32 + lane;
+      const bool live = s.channel < p.n;
       const int width = GATED ? 2 * p.n : p.n;
-      const int row = GATED && lane >= 16 ? p.n + channel : channel;
-      const float sb = live ? __ldg(p.b_scales + static_cast<long long>(tile.expert) * width + row) : 0.0f;
-      const float bias = live && p.bias != nullptr ? __ldg(p.bias + row) : 0.0f;
-      // Its tokens: all of the tile's, or with a split this CTA's share; their scales are fetched while
-      // the MMAs run.
-      const int c_begin = p.split > 1 ? tile.columns * static_cast<int>(rank) / p.split : 0;
-      const int c_end = min(p.split > 1 ? tile.columns * (static_cast<int>(rank) + 1) / p.split : tile.columns,
-                            tile.tokens);
-      for (int c = c_begin + 32 * part, i = 0; c < c_end; c += 32 * parts, i += 32) {
-        sa_stage[i + lane] = c + lane < c_end ? __ldg(p.a_scales + tile.m0 + c + lane) : 0.0f;
+      const int row = GATED && lane >= 16 ? p.n + s.channel : s.channel;
+      s.sb = live ? __ldg(p.b_scales + static_cast<long long>(s.tile.expert) * width + row) : 0.0f;
+      s.bias = live && p.bias != nullptr ? __ldg(p.bias + row) : 0.0f;
+      s.c_begin = p.split > 1 ? s.tile.columns * static_cast<int>(rank) / p.split : 0;
+      s.c_end = min(p.split > 1 ? s.tile.columns * (static_cast<int>(rank) + 1) / p.split : s.tile.columns,
+                    s.tile.tokens);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int c = s.c_begin + 32 * (part + i * parts) + lane;
+        s.sa[i] = c < s.c_end ? __ldg(p.a_scales + s.tile.m0 + c) : 0.0f;
       }
+      return s;
+    };
+    uint32_t acc = 0, acc_phase = 0;
+    Share next{};
+    if (first_tile < tiles) next = share_of(first_tile);
+    for (uint32_t t = first_tile; t < tiles; t += step) {
+      const Int8Tile tile = next.tile;
+      const int channel = next.channel, c_begin = next.c_begin, c_end = next.c_end;
+      const bool live = channel < p.n;
+      const float sb = next.sb, bias = next.bias;
+      sa_stage[lane] = next.sa[0];
+      sa_stage[32 + lane] = next.sa[1];
+      // The next tile's scales are on their way while this tile's MMAs run and its results leave: each
+      // tile fetching its own takes 44 us for 8192 x 8192 x 256, this 39.5.
+      if (t + step < tiles) next = share_of(t + step);
       __syncwarp();
       if (!mbar_wait(smem_u32(&bar_acc_full[acc]), acc_phase, abort_ptr)) {
         int8_give_up(abort_ptr, kInt8EpilogueTimeout);
@@ -587,6 +642,25 @@ int8_tile_kernel(const __grid_constant__ Int8TileParams p) {
             y[i] = up_lane ? silu(other) * mine : silu(mine) * other;
           }
           const int parity = up_lane ? 1 : 0;
+          if (p.staged && count == 32) {
+            // A token's 16 channels are 32 bytes of the box.
+            const uint32_t box = staging + static_cast<uint32_t>(warp - 2) * kInt8StagedBytes;
+            const uint32_t to = box + static_cast<uint32_t>(parity * 32 + (lane & 15) * 2);
+            if (lane == 0) bulk_wait_group_read_all();
+            __syncwarp();
+            if (p.out_kind == 0) {
+              stage_columns<__half>(to, 64, y);
+            } else {
+              stage_columns<__nv_bfloat16>(to, 64, y);
+            }
+            fence_proxy_async_shared();
+            __syncwarp();
+            if (lane == 0 && channel < p.n) {
+              tma_store_rows(&p.map_d, box, channel, tile.m0 + c);
+              bulk_commit_group();
+            }
+            continue;
+          }
           const long long first = (tile.m0 + c + parity) * p.ldd + channel;
           const int mine = live ? (count - parity + 1) / 2 : 0;
           if (p.out_kind == 0) {
@@ -597,6 +671,24 @@ int8_tile_kernel(const __grid_constant__ Int8TileParams p) {
             store_columns(static_cast<__nv_bfloat16*>(p.d) + first, 2 * p.ldd, y, mine);
           }
         } else {
+          if (p.staged && count == 32) {
+            const uint32_t box = staging + static_cast<uint32_t>(warp - 2) * kInt8StagedBytes;
+            const uint32_t to = box + static_cast<uint32_t>(lane * 2);
+            if (lane == 0) bulk_wait_group_read_all();
+            __syncwarp();
+            if (p.out_kind == 0) {
+              stage_columns<__half>(to, 64, v);
+            } else {
+              stage_columns<__nv_bfloat16>(to, 64, v);
+            }
+            fence_proxy_async_shared();
+            __syncwarp();
+            if (lane == 0 && channel < p.n) {
+              tma_store_rows(&p.map_d, box, channel, tile.m0 + c);
+              bulk_commit_group();
+            }
+            continue;
+          }
           const long long first = (tile.m0 + c) * p.ldd + channel;
           const int mine = live ? count : 0;
           if (p.out_kind == 0) {
@@ -620,6 +712,8 @@ int8_tile_kernel(const __grid_constant__ Int8TileParams p) {
       acc ^= 1u;
       if (acc == 0) acc_phase ^= 1u;
     }
+    // The staging outlives the last stores' reads of it.
+    if (p.staged && lane == 0) bulk_wait_group_read_all();
   }
 
   tc_fence_before_sync();

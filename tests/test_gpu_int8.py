@@ -164,6 +164,41 @@ def test_grouped_product(counts, n, k, gated):
                 assert_product(out[lo:hi], a[lo:hi], b[e], sa[lo:hi], sb[e], None, gated)
 
 
+@pytest.mark.parametrize("n", [1304, 1305])
+@pytest.mark.parametrize("k", [1, 200, 1024, 1040])
+@pytest.mark.parametrize("gated", [False, True])
+def test_shallow_products_of_several_tiles_a_cta(n, k, gated):
+    """More tiles than the GPU has SMs, of a small depth: however D lies (rows on multiples of eight
+    elements or not) the bits are the same and nothing beside them is written; in groups too, whose last
+    rows end inside a tile."""
+    g = rng_of(n + k)
+    width, rows = 2 * n if gated else n, 5003
+    a, b = make_codes(g, rows, k), make_codes(g, 2, width, k)
+    sa = 0.5 + torch.rand(rows, device=DEV, generator=g)
+    sb = (0.5 + torch.rand((2, width), device=DEV, generator=g)) * (2e-4 / k ** 0.5)
+    bias = torch.randn(width, device=DEV, generator=g)
+    offsets = torch.tensor([7, 2606, rows - 9], dtype=torch.int32, device=DEV)
+    for dtype in (torch.bfloat16, torch.float16):
+        dense, grouped = [], []
+        for pitch in (-(-n // 8) * 8, n + 16 + -n % 8, n + 5):
+            out, check = guarded(rows, n, dtype, pitch=pitch)
+            dense.append(int8.gemm(a, b[0], sa, sb[0], bias=bias, gated=gated, out_dtype=dtype, out=out).clone())
+            check()
+            out, check = guarded(rows, n, dtype, pitch=pitch)
+            int8.grouped_gemm(a, b, sa, sb, offsets, gated=gated, out_dtype=dtype, out=out)
+            check()
+            assert (out[:7] == 77.0).all() and (out[rows - 9:] == 77.0).all()
+            grouped.append(out.clone())
+        assert_product(dense[0], a, b[0], sa, sb[0], bias, gated)
+        for e, (lo, hi) in enumerate(((7, 2606), (2606, rows - 9))):
+            assert_product(grouped[0][lo:hi], a[lo:hi], b[e], sa[lo:hi], sb[e], None, gated)
+        for other in dense[1:]:
+            assert torch.equal(other, dense[0])
+        for other in grouped[1:]:
+            assert torch.equal(other, grouped[0])
+    int8.check_status(DEV)
+
+
 @pytest.mark.parametrize("rows", [32, 64, 96, 128, 256, 512])
 def test_one_expert_that_owns_few_of_the_rows(rows):
     """The tile is made for all rows of the buffers, the group has fewer: its MMA is narrower than
