@@ -294,6 +294,8 @@ int8_tile_kernel(const __grid_constant__ Int8TileParams p) {
       asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
     }
   }
+  // What the kernel before writes is read behind this, by plain loads: the read-only path (__ldg) is for
+  // memory that nothing writes while the kernel is resident, and this one may be resident early.
   grid_dependency_wait();
   grid_launch_dependents();
   if (warp == 0) {
@@ -303,8 +305,8 @@ int8_tile_kernel(const __grid_constant__ Int8TileParams p) {
     int before = 0, last_row = 0;
     for (int e0 = 0; e0 < p.experts; e0 += 32) {
       const int e = e0 + lane;
-      int row = e < p.experts ? (p.offsets != nullptr ? __ldg(p.offsets + e) : 0) : 0;
-      int next = e < p.experts ? (p.offsets != nullptr ? __ldg(p.offsets + e + 1) : p.rows) : 0;
+      int row = e < p.experts ? (p.offsets != nullptr ? p.offsets[e] : 0) : 0;
+      int next = e < p.experts ? (p.offsets != nullptr ? p.offsets[e + 1] : p.rows) : 0;
       row = min(max(row, last_row), p.rows);
       next = min(max(next, row), p.rows);
 #pragma unroll
@@ -544,15 +546,15 @@ int8_tile_kernel(const __grid_constant__ Int8TileParams p) {
       const bool live = s.channel < p.n;
       const int width = GATED ? 2 * p.n : p.n;
       const int row = GATED && lane >= 16 ? p.n + s.channel : s.channel;
-      s.sb = live ? __ldg(p.b_scales + static_cast<long long>(s.tile.expert) * width + row) : 0.0f;
-      s.bias = live && p.bias != nullptr ? __ldg(p.bias + row) : 0.0f;
+      s.sb = live ? p.b_scales[static_cast<long long>(s.tile.expert) * width + row] : 0.0f;
+      s.bias = live && p.bias != nullptr ? p.bias[row] : 0.0f;
       s.c_begin = p.split > 1 ? s.tile.columns * static_cast<int>(rank) / p.split : 0;
       s.c_end = min(p.split > 1 ? s.tile.columns * (static_cast<int>(rank) + 1) / p.split : s.tile.columns,
                     s.tile.tokens);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int c = s.c_begin + 32 * (part + i * parts) + lane;
-        s.sa[i] = c < s.c_end ? __ldg(p.a_scales + s.tile.m0 + c) : 0.0f;
+        s.sa[i] = c < s.c_end ? p.a_scales[s.tile.m0 + c] : 0.0f;
       }
       return s;
     };

@@ -324,7 +324,8 @@ struct QuantizeParams {
 };
 
 // Row r of the codes = row source[r] (or r) of x. A source row outside [0, tokens) leaves the
-// row's codes and its scale as they were.
+// row's codes and its scale as they were. Plain loads: the kernel may be resident while the one before
+// writes what it reads.
 template <bool WIDE, int P, int N, int THREADS, bool WARP>
 __global__ void __maxnreg__(row_registers(false, P, N, THREADS, WARP)) int8_quantize_kernel(const QuantizeParams p) {
   __shared__ uint32_t maxima[32];
@@ -332,7 +333,7 @@ __global__ void __maxnreg__(row_registers(false, P, N, THREADS, WARP)) int8_quan
   grid_launch_dependents();
   const int r = row_of_thread<WARP>();
   if (r >= p.rows) return;
-  const int t = p.source != nullptr ? __ldg(p.source + r) : r;
+  const int t = p.source != nullptr ? p.source[r] : r;
   if (t < 0 || t >= p.tokens) return;
   const int step = P * (WARP ? 32 : P == 1 ? THREADS : blockDim.x);
   const int first = P * (WARP ? threadIdx.x & 31 : threadIdx.x);
@@ -582,7 +583,7 @@ __device__ __forceinline__ float load_kind(const void* p, long long i, int kind)
 __global__ void __launch_bounds__(1024) int8_quantize_long_kernel(const QuantizeParams p) {
   __shared__ uint32_t maxima[32];
   const int r = blockIdx.x;
-  const int t = p.source != nullptr ? __ldg(p.source + r) : r;
+  const int t = p.source != nullptr ? p.source[r] : r;
   if (t < 0 || t >= p.tokens) return;
   uint32_t amax = 0;
 #pragma unroll 8
