@@ -215,7 +215,7 @@ def quantize_tokens(x: torch.Tensor, *, rows: torch.Tensor | None = None,
     ``[R]`` on the device) gathers: row r of the codes is row ``rows[r]`` of ``x``; an index outside
     ``[0, tokens)`` leaves row r as it was. ``out``: codes and scales to write to."""
     index = x.get_device()
-    if x.requires_grad and torch.is_grad_enabled():
+    if torch.is_grad_enabled() and (x.requires_grad or (out is not None and out[1].requires_grad)):
         _refuse_gradients()
     kind = IN_KINDS.get(x.dtype)
     if x.dim() != 2 or kind is None:
@@ -263,7 +263,7 @@ def residual_norm(x: torch.Tensor, residual: torch.Tensor | None = None, *,
     Returns ``(r, y, scales)``: ``r`` in the residual's type, ``y`` (of the unrounded ``r``) in
     ``out_dtype`` (default: the residual's type) or, with ``quantize``, as INT8 codes with their
     ``scales``; what is not made is None. ``gate`` is ``[hidden]`` or ``[gates, hidden]``, each row
-    for ``tokens / gates`` consecutive tokens. Weights and gate are FP32. Without a residual only
+    for ``tokens / gates`` consecutive tokens. Weights and gate are FP32, ``eps`` is above zero. Without a residual only
     ``y = x / rms(x) * next_weight`` is made. ``residual_out`` (may be ``residual`` itself) and ``out``
     (``y``, or codes and scales) are tensors to write to."""
     index, device = x.get_device(), x.device
@@ -271,7 +271,8 @@ def residual_norm(x: torch.Tensor, residual: torch.Tensor | None = None, *,
             x.requires_grad or (residual is not None and residual.requires_grad)
             or (post_weight is not None and post_weight.requires_grad) or (gate is not None and gate.requires_grad)
             or (next_weight is not None and next_weight.requires_grad)
-            or (residual_out is not None and residual_out.requires_grad)):
+            or (residual_out is not None and residual_out.requires_grad)
+            or (out is not None and any(t.requires_grad for t in (out if quantize else (out,))))):
         _refuse_gradients()
     x_kind = IN_KINDS.get(x.dtype)
     if x.dim() != 2 or x_kind is None:

@@ -554,6 +554,8 @@ class Int8MoELayer:
             raise ValueError("activations, ids and weights do not match")
         if any(t.device != self.device for t in (x, topk_ids, topk_weights)):
             raise ValueError("operands must be on the layer's device")
+        if torch.is_grad_enabled() and (x.requires_grad or topk_weights.requires_grad):
+            raise ValueError("the INT8 layer has no backward; call it under torch.no_grad()")
         pairs = tokens * choices
         out = torch.empty((tokens, self.hidden), dtype=torch.float32, device=self.device)
         if pairs == 0:

@@ -658,6 +658,35 @@ def test_int8_layer_against_its_stages(tokens, hidden, inter, experts, choices, 
         layer.forward(x[:, :-16], ids, weights)
 
 
+@pytest.mark.parametrize("tokens", [1, 2, 130, 3000])
+def test_int8_layer_of_uneven_routings(tokens):
+    """The same expert twice in a token, every token at one expert, ids on both sides of the experts,
+    rows of a wider buffer: each equals the layer's stages, and two streams equal one."""
+    layer, x, ids, weights = moe_case(tokens, 256, 96, 6, 3)
+    wide = torch.full((tokens, 256 + 24), float("nan"), device=DEV, dtype=x.dtype)
+    wide[:, 8:264] = x
+    for one in (torch.zeros_like(ids), torch.full_like(ids, 5), ids.clone()):
+        one[0, 1:] = one[0, 0]
+        assert_moe(layer.forward(wide[:, 8:264], one, weights), x, one, weights, layer)
+        one[tokens // 2, 0], one[tokens // 3, 1] = -1, 1 << 40
+        want = layer.forward(x, one, weights)
+        assert_moe(want, x, one, weights, layer)
+        streams = [torch.cuda.Stream() for _ in range(2)]
+        torch.cuda.synchronize()
+        got = []
+        for turn in range(6):
+            with torch.cuda.stream(streams[turn % 2]):
+                got.append(layer.forward(x, one, weights))
+        torch.cuda.synchronize()
+        for other in got:
+            assert torch.equal(other, want)
+    with pytest.raises(ValueError):
+        layer.forward(x, ids, weights.clone().requires_grad_())
+    with torch.no_grad():
+        layer.forward(x, ids, weights.clone().requires_grad_())
+    int8.check_status(DEV)
+
+
 def test_int8_block_chain_in_a_graph():
     """Two blocks, the first's last norm fused with the second's first, captured and replayed on new
     tokens, equal the same operators called one by one."""

@@ -60,6 +60,8 @@ def test_functions_refuse_what_they_cannot_take():
         lambda: int8.residual_norm(ones(4, 8), ones(4, 8), next_weight=ones(8), quantize=True,
                                    out_dtype=torch.float16),
         lambda: int8.residual_norm(ones(4, 8), next_weight=ones(8), residual_out=ones(4, 8)),
+        lambda: int8.residual_norm(ones(4, 8), next_weight=ones(8), out=ones(4, 8).requires_grad_()),
+        lambda: int8.quantize_tokens(ones(4, 16), out=(codes(4, 16), ones(4).requires_grad_())),
     ):
         with pytest.raises(ValueError):
             call()
