@@ -4,6 +4,7 @@
 #include "../../include/nvfp4_b200.h"
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstdint>
 #include <cstdio>
@@ -127,35 +128,73 @@ struct Tiling {
   int ctas, tile_tokens, sub, split;
 };
 
+// Clusters of `split` CTAs, one to an SM, that the current device holds at once: clusters do not reach
+// over its groups of SMs, which are not all of one size (B200: 74 of two, 33 of four, 15 of eight). A
+// property of the device, asked for once.
+int cluster_slots(int split, int sms) {
+  static std::atomic<int> known[64][4];
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess || device >= 64) return sms / split * 3 / 4;
+  std::atomic<int>& slot = known[device][split == 2 ? 1 : split == 4 ? 2 : 3];
+  int count = slot.load(std::memory_order_relaxed);
+  if (count > 0) return count;
+  const void* kernel = reinterpret_cast<const void*>(tile_kernel(1, 2, false));
+  cudaLaunchAttribute attribute[1];
+  attribute[0].id = cudaLaunchAttributeClusterDimension;
+  attribute[0].val.clusterDim.x = static_cast<unsigned int>(split);
+  attribute[0].val.clusterDim.y = 1;
+  attribute[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(static_cast<unsigned int>(split));
+  config.blockDim = dim3(int8_threads(32));
+  config.dynamicSmemBytes = kSharedLimit;
+  config.attrs = attribute;
+  config.numAttrs = 1;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSharedLimit) != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&count, kernel, &config) != cudaSuccess || count < 1) {
+    cudaGetLastError();
+    return sms / split * 3 / 4;
+  }
+  slot.store(count, std::memory_order_relaxed);
+  return count;
+}
+
 // Microseconds of a tiling by the measured costs of its parts (1.9 GHz):
 //   a step of 128 k   the largest of its loads (140 GB/s an SM), its MMAs (2 columns a clock; 4 x 32 k)
-//                     and the loops that issue them (0.135 us; with one piece a stage 0.2 us)
-//   a tile            its steps, or, where those are shorter, its epilogue: 1 us for every 32 tokens
-//                     of a warp; the last epilogue stands alone
-//   a pair            0.5 us for its cluster; a split 1.2 us and 0.02 us a token for the exchange of
-//                     partial sums
+//                     and the loops that issue them (0.135 us; with one piece a stage 0.22 us)
+//   a tile            its steps or, where those are shorter, its epilogue: 0.6 us and 0.3 for every 32
+//                     tokens, gated 0.7 and 0.53; the first tile's steps or the last one's epilogue
+//                     stand alone
+//   a pair            0.5 us for its cluster; a split 0.5 us, 0.6 for every 32 tokens and 0.1 for
+//                     each part for the exchange of partial sums
 //   everything        not less than the operands' bytes at 6 TB/s; and a tenth of the loads at 12 TB/s,
 //                     which decides between tilings that are otherwise alike
+// Groups differ in size: 0.6 of a tile each is counted for their last ones.
 // What the choice is worth (device time, rows x n x k): 256 x 4096 x 7168 takes 13.4 us in pairs on 64
-// tokens and 21.9 on 256, where 32 of 148 SMs work; 200 x 5120 x 5120 11.7 on 96 and 18.0 on 256; 16 x
-// 7168 x 2048 6.3 us with all of k in one CTA and 8.0 split in two; 32 x 4096 x 8192 11.6 split in four
-// and 23 whole; 16 experts of 8192 rows, gated 1536 x 4096, 93 in pairs on 256 tokens and 270 on 32.
+// tokens and 21.9 on 256, where 32 of 148 SMs work; 16 x 7168 x 2048 6.3 us with all of k in one CTA and
+// 7.3 split in two; 32 x 4096 x 8192 9.6 split in four and 23 whole; 277 x 256 x 5136 8.0 split in four,
+// 12.8 whole and 14.3 in eight, whose clusters find no room together; 16 experts of 8192 rows, gated 1536
+// x 4096, 92 in pairs on 256 tokens, 98 on 192 and 270 on 32; 2 experts of 3303 rows, 352 x 4384, 11.7
+// on 96 and 16.4 on 256.
 double tiling_us(const Product& q, const Tiling& t, int sms, double* tiles) {
   const int groups = std::min(q.experts, q.rows);
   const int per_group = (q.rows + groups - 1) / groups;
-  const int m_tiles = (per_group + t.tile_tokens - 1) / t.tile_tokens;
-  const int columns = ((per_group + m_tiles - 1) / m_tiles + 31) / 32 * 32;
+  const double m_tiles = q.experts == 1 ? (q.rows + t.tile_tokens - 1) / t.tile_tokens
+                                        : std::max<double>(groups, static_cast<double>(q.rows) / t.tile_tokens +
+                                                                       0.6 * groups);
+  const int columns = std::min<long long>(t.tile_tokens, ((q.experts == 1 ? 1ll : 2ll) * per_group + 31) / 32 * 32);
   const int channels = (q.gated ? 64 : 128) * t.ctas;
-  *tiles = static_cast<double>(groups) * m_tiles * ((q.n + channels - 1) / channels);
+  *tiles = m_tiles * ((q.n + channels - 1) / channels);
   const double loads = (128.0 + static_cast<double>(columns) / t.ctas) * 128.0 / 140e3;
   const double mmas = columns * 2.0 / 1900.0;
-  const double step = std::max(std::max(loads, mmas), t.sub == 2 ? 0.135 : 0.2);
   const int chunks = columns / 32;
-  const double epilogue = (chunks + int8_parts(t.tile_tokens) - 1) / int8_parts(t.tile_tokens);
+  const double epilogue = q.gated ? 0.7 + 0.53 * chunks : 0.6 + 0.3 * chunks;
   const int k_tiles = (q.k + 127) / 128;
-  const double rounds = std::ceil(*tiles * t.split / (sms / t.ctas));
-  const double work = rounds * std::max((k_tiles + t.split - 1) / t.split * step, epilogue) + epilogue +
-                      (t.ctas == 2 ? 0.5 : 0.0) + (t.split > 1 ? 1.2 + 0.02 * columns : 0.0);
+  const double steps = (k_tiles + t.split - 1) / t.split *
+                       std::max(std::max(loads, mmas), t.sub == 2 ? 0.135 : 0.22);
+  const double rounds = t.split > 1 ? 1.0 : std::ceil(*tiles / (sms / t.ctas));
+  const double work = rounds * std::max(steps, epilogue) + std::min(steps, epilogue) +
+                      (t.ctas == 2 ? 0.5 : 0.0) + (t.split > 1 ? 0.5 + 0.6 * chunks + 0.1 * t.split : 0.0);
   const double width = q.gated ? 2.0 * q.n : q.n;
   const double bytes = groups * width * q.k + static_cast<double>(q.rows) * (q.k + 2.0 * q.n);
   const double loaded = *tiles * k_tiles * (128.0 * t.ctas + columns) * 128.0;
@@ -165,19 +204,19 @@ double tiling_us(const Product& q, const Tiling& t, int sms, double* tiles) {
 Tiling choose_tiling(const Product& q, int sms) {
   const int groups = std::min(q.experts, q.rows);
   const int per_group = (q.rows + groups - 1) / groups;
-  // Groups differ in size: a tile that holds twice the average reads few weights twice.
-  const int widest = std::min(256, (per_group + 31) / 32 * 32);
-  const int narrowest = q.experts > 1 ? std::min(256, (2 * per_group + 31) / 32 * 32) : 32;
+  // Of groups a tile up to twice the average: what is larger takes several.
+  const int widest = static_cast<int>(
+      std::min<long long>(256, ((q.experts == 1 ? 1ll : 2ll) * per_group + 31) / 32 * 32));
   Tiling best{};
   double best_us = 0.0;
   for (int ctas = per_group > 32 ? 2 : 1; ctas >= 1; --ctas) {
-    const int least = std::max(narrowest, 32 * ctas);
-    for (int tokens = std::max(widest, least); tokens >= least; tokens -= 32) {
+    for (int tokens = widest; tokens >= 32 * ctas; tokens -= 32) {
       for (int split = 1; split <= (ctas == 1 ? 8 : 1); split *= 2) {
         const Tiling t{ctas, tokens, ctas == 1 || tokens <= 128 ? 2 : 1, split};
         double tiles = 0.0;
         const double us = tiling_us(q, t, sms, &tiles);
-        if (split > 1 && (tiles * split > sms || split * 2 > (q.k + 127) / 128)) break;
+        // A split tile is a cluster's only one: all of them run at once.
+        if (split > 1 && (split * 2 > (q.k + 127) / 128 || tiles > cluster_slots(split, sms))) break;
         if (best.ctas == 0 || us < best_us * 0.98) {
           best = t;
           best_us = us;
@@ -314,8 +353,11 @@ void launch_rows(void (*kernel)(Params), int blocks, int threads, cudaStream_t s
   (void)cudaLaunchKernelExC(&config, reinterpret_cast<const void*>(kernel), args);
 }
 
-// How rows of `width` elements lie over threads. A warp to a row up to 1,024 elements, where there
-// are rows enough; else a CTA. In pieces of eight: few threads with much work where there are many
+// How rows of `width` elements lie over threads. A warp to a row up to `warp_width` elements, where there
+// are rows enough; else a CTA. The quantiser in pieces of eight takes warps up to 1,024 elements (8192 x
+// 1000: 5.9 us, with CTAs 9.1); the others only up to 256, since a lane with 32 elements and their
+// 64-bit sums takes longer than a CTA's barriers (norms of 2900 x 370: 8.7 us, with warps 19; 8192 x 1000
+// 15.5 and 17.7; 8192 x 101 7.7 and with CTAs 24; codes of 4000 x 945 6.2, with warps 8.1). In pieces of eight: few threads with much work where there are many
 // rows (`elements` a thread: fewer, and the fixed cost of a row's reductions shows), many threads
 // where there are too few to fill the SMs (a row's latency is what counts then). One at a time: 8
 // elements a thread, or what 1,024 threads need.
@@ -326,9 +368,9 @@ struct RowGrid {
 
 constexpr int kMaxRegisterRow = 32768;
 
-RowGrid row_grid(int rows, int width, int p, int elements) {
+RowGrid row_grid(int rows, int width, int p, int elements, int warp_width) {
   RowGrid g{};
-  g.warp = width <= 1024 && rows > host_sm_count();
+  g.warp = width <= warp_width && rows > host_sm_count();
   if (g.warp) {
     g.elements = width <= 256 ? 8 : 32;
     g.threads = 32 * kWarpRows;
@@ -359,8 +401,10 @@ void launch_quantize(const RowGrid& g, cudaStream_t s, const QuantizeParams& p) 
   constexpr int kWarps = 32 * kWarpRows;
   void (*kernel)(QuantizeParams);
   if (g.warp) {
-    kernel = g.elements == 8 ? int8_quantize_kernel<WIDE, P, 8 / P, kWarps, true>
-                             : int8_quantize_kernel<WIDE, P, 32 / P, kWarps, true>;
+    kernel = int8_quantize_kernel<WIDE, P, 8 / P, kWarps, true>;
+    if constexpr (P == 8) {
+      if (g.elements == 32) kernel = int8_quantize_kernel<WIDE, 8, 4, kWarps, true>;
+    }
   } else if constexpr (P == 1) {
     kernel = g.threads == 128   ? int8_quantize_kernel<WIDE, 1, 8, 128, false>
              : g.threads == 256 ? int8_quantize_kernel<WIDE, 1, 8, 256, false>
@@ -384,8 +428,7 @@ void launch_norm(const RowGrid& g, cudaStream_t s, const NormParams& p) {
   constexpr int kWarps = 32 * kWarpRows;
   void (*kernel)(NormParams);
   if (g.warp) {
-    kernel = g.elements == 8 ? residual_norm_kernel<X_WIDE, R_WIDE, P, 8 / P, kWarps, true>
-                             : residual_norm_kernel<X_WIDE, R_WIDE, P, 32 / P, kWarps, true>;
+    kernel = residual_norm_kernel<X_WIDE, R_WIDE, P, 8 / P, kWarps, true>;
   } else if constexpr (P == 1) {
     kernel = g.threads == 128   ? residual_norm_kernel<X_WIDE, R_WIDE, 1, 8, 128, false>
              : g.threads == 256 ? residual_norm_kernel<X_WIDE, R_WIDE, 1, 8, 256, false>
@@ -483,10 +526,10 @@ int nvfp4_int8_quantize(const void* x, int x_kind, long long ldx, const int* sou
     int8_quantize_long_kernel<<<rows, 1024, 0, s>>>(p);
   } else if (k % 8 == 0 && rows_in_eights(x, ldx, kind_bytes(x_kind), tokens) &&
              rows_in_eights(q, ldq, 1, rows)) {
-    const RowGrid g = row_grid(rows, k, 8, 32);
+    const RowGrid g = row_grid(rows, k, 8, 32, 1024);
     if (x_kind == NVFP4_IN_F32) launch_quantize<true, 8>(g, s, p); else launch_quantize<false, 8>(g, s, p);
   } else {
-    const RowGrid g = row_grid(rows, k, 1, 32);
+    const RowGrid g = row_grid(rows, k, 1, 32, 256);
     if (x_kind == NVFP4_IN_F32) launch_quantize<true, 1>(g, s, p); else launch_quantize<false, 1>(g, s, p);
   }
   CUDA_TRY(cudaGetLastError());
@@ -563,9 +606,9 @@ int nvfp4_residual_norm(const void* x, int x_kind, long long ldx, const void* re
       rows_in_eights(r, ldr, r_bytes, tokens) && rows_in_eights(post_weight, 0, 4, 1) &&
       rows_in_eights(gate, hidden, 4, gates) &&
       (next_weight == nullptr || (rows_in_eights(next_weight, 0, 4, 1) && rows_in_eights(y, ldy, y_bytes, tokens)))) {
-    launch_norm<8>(row_grid(tokens, hidden, 8, 16), s, p);
+    launch_norm<8>(row_grid(tokens, hidden, 8, 16, 256), s, p);
   } else {
-    launch_norm<1>(row_grid(tokens, hidden, 1, 16), s, p);
+    launch_norm<1>(row_grid(tokens, hidden, 1, 16, 256), s, p);
   }
   CUDA_TRY(cudaGetLastError());
   return 0;

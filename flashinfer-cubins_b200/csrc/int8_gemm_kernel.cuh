@@ -601,12 +601,19 @@ int8_tile_kernel(const __grid_constant__ Int8TileParams p) {
         if (p.split > 1) {
 #pragma unroll
           for (int i = 0; i < 32; ++i) r[i] = 0;
-          for (int s = 0; s < p.split; ++s) {
-            const uint32_t from = cluster_map_shared(
-                smem_base + static_cast<uint32_t>(c * 128 + quarter * 32 + lane) * 4u, s);
+          // Eight tokens at a time from all parts, the loads of four parts under way together (3 x 96 x
+          // 6832 split in eight: one part after the other 9.5 us, this 6.4).
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              if (i < count) r[i] += static_cast<uint32_t>(ld_cluster_s32(from + i * 512));
+          for (int i0 = 0; i0 < 32; i0 += 8) {
+            if (i0 >= count) break;
+#pragma unroll 4
+            for (int s = 0; s < p.split; ++s) {
+              const uint32_t from = cluster_map_shared(
+                  smem_base + static_cast<uint32_t>((c + i0) * 128 + quarter * 32 + lane) * 4u, s);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                if (i0 + i < count) r[i0 + i] += static_cast<uint32_t>(ld_cluster_s32(from + i * 512));
+              }
             }
           }
         } else {

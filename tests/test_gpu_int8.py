@@ -98,6 +98,33 @@ def test_product_over_sizes(m, n, k, gated):
         assert torch.equal(again, got), "the same call gave other bits"
 
 
+@pytest.mark.parametrize("m,n,k", [(3, 96, 6832), (277, 256, 5136), (313, 416, 1500), (33, 130, 2049), (842, 40, 9008),
+                                   (120, 24, 640), (60, 300, 4097), (2297, 585, 300)])
+@pytest.mark.parametrize("gated", [False, True])
+def test_products_of_few_tiles_and_great_depth(m, n, k, gated):
+    """Few tiles: parts of k on several CTAs, whose integer sums give the bits of the same rows beside
+    others (other tiles, other parts)."""
+    g = rng_of(m + n + k)
+    width = 2 * n if gated else n
+    a, b = make_codes(g, m + 300, k), make_codes(g, width, k)
+    sa = 0.5 + torch.rand(m + 300, device=DEV, generator=g)
+    sb = (0.5 + torch.rand(width, device=DEV, generator=g)) * (2e-4 / k ** 0.5)
+    for dtype in DTYPES:
+        out, check = guarded(m, n, dtype)
+        int8.gemm(a[:m], b, sa[:m], sb, gated=gated, out_dtype=dtype, out=out)
+        check()
+        assert_product(out, a[:m], b, sa[:m], sb, None, gated)
+        for rows in (1, m // 2 + 1, m + 300):
+            other = int8.gemm(a[:rows], b, sa[:rows], sb, gated=gated, out_dtype=dtype)
+            assert torch.equal(other[:m], out[:rows])
+        counts = torch.tensor([0, m // 3, m // 3, m], dtype=torch.int32, device=DEV)
+        grouped = int8.grouped_gemm(a[:m], b.expand(1, width, k).repeat(3, 1, 1) if k % 16 == 0 else make_codes(g, 3, width, k),
+                                    sa[:m], sb.repeat(3, 1), counts, gated=gated, out_dtype=dtype)
+        if k % 16 == 0:
+            assert torch.equal(grouped, out)
+    int8.check_status(DEV)
+
+
 def test_product_extremes():
     """All codes -128 at a depth near the largest: the 32-bit sum does not wrap, and FP32 output
     is it times the scales, rounded as written. Zero, infinite and NaN scales go through."""
