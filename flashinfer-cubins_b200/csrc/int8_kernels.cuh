@@ -271,12 +271,14 @@ __device__ __forceinline__ void store_codes(int8_t* row, int c, const float (&v)
 // the issue slots idle with three), so they get fewer than the compiler would take: the norms in pieces
 // of eight 48 (8192 x 5120: 70 us, with 64 registers 78, with 40 and spills 73), the quantiser 40 (8192 x
 // 7168: 31.8 us, with 52 registers 32.4), rows taken one element at a time 40 (4096 x 3001 to codes: 43
-// us, with 64 registers 53). CTAs of 1,024 threads and threads of 32 single elements need 64.
+// us, with 64 registers 53; codes of 8192 x 7169 76, with 64 registers 90). CTAs of 1,024 threads need 64, and
+// the norms' threads of 16 single elements do no better with fewer.
 constexpr int row_registers(bool norm, int p, int n, int threads, bool warp) {
   const int elements = p * n;
   if (elements == 8) return p == 1 ? 40 : threads == 1024 ? 64 : 48;
-  if (warp) return norm ? 64 : 48;
-  if (p == 8 && threads == 512) return !norm ? 40 : n == 2 ? 48 : 64;
+  if (warp) return 48;  // of the quantiser alone
+  if (!norm && threads == 512) return 40;
+  if (p == 8 && threads == 512) return n == 2 ? 48 : 64;
   return 64;
 }
 
