@@ -275,9 +275,9 @@ int launch_product(const Product& q, void* stream) {
     p.map_a_part = p.map_a;
   }
   // 16-bit results leave through shared memory where the MMAs do not hide a store of 64 bytes a warp and
-  // CTAs take several tiles: 8192 x 8192 x 64 takes 41.4 us against 49.3 with direct stores, k = 256 35
-  // against 39.5, gated 4096 x 8192 x 256 55.4 against 58.5; k = 1024 57 against 58; k = 2048 95.0
-  // against 93.6. A CTA's only tile gains nothing: 300 x 4096 x 256 5.2 us against 5.0. The copies
+  // CTAs take several tiles: 8192 x 8192 x 64 takes 32.3 us against 38.6 with direct stores, k = 256 33.9
+  // against 39.6, gated 4096 x 8192 x 256 59.9 against 62.6; k = 1024 56.8 against 57.7; k = 2048 92.8
+  // against 91.1. A CTA's only tile gains nothing: 300 x 4096 x 256 4.9 us against 4.7. The copies
   // write 16 bytes at a time, so rows of D must start, follow and end on multiples of eight.
   const long long walkers = sms / ctas;
   p.staged = q.out_kind != NVFP4_OUT_F32 && q.k <= 1024 && split == 1 && tiles > walkers && q.n % 8 == 0 &&

@@ -342,7 +342,7 @@ int8_tile_kernel(const __grid_constant__ Int8TileParams p) {
   const int m_tiles = tiles_before[p.experts];
   const int n_tiles = (p.n + channels * CTAS - 1) / (channels * CTAS);
   // 32 bits hold every tile's number (the host checks): the divisions below are done by every warp for
-  // every tile, and with 64-bit ones 8192 x 8192 x 64 takes 42.3 us for 41.4.
+  // every tile, and 64-bit ones cost 8192 x 8192 x 64 0.9 us.
   const uint32_t tiles = static_cast<uint32_t>(m_tiles) * static_cast<uint32_t>(n_tiles);
   const int group = p.split > 1 ? p.split : CTAS;  // CTAs that share a tile
   const uint32_t first_tile = blockIdx.x / group;
