@@ -162,8 +162,8 @@ int cluster_slots(int split, int sms) {
 // Microseconds of a tiling by the measured costs of its parts (1.9 GHz):
 //   a step of 128 k   the largest of its loads (140 GB/s an SM), its MMAs (2 columns a clock; 4 x 32 k)
 //                     and the loops that issue them (0.135 us; with one piece a stage 0.22 us)
-//   a tile            its steps or, where those are shorter, its epilogue: 0.6 us and 0.3 for every 32
-//                     tokens, gated 0.7 and 0.53; the first tile's steps or the last one's epilogue
+//   a tile            its steps or, where those are shorter, its epilogue: 0.6 us and 0.3 (gated
+//                     0.33) for every 32 tokens; the first tile's steps or the last one's epilogue
 //                     stand alone
 //   a pair            0.5 us for its cluster; a split 0.5 us, 0.6 for every 32 tokens and 0.1 for
 //                     each part for the exchange of partial sums
@@ -188,7 +188,7 @@ double tiling_us(const Product& q, const Tiling& t, int sms, double* tiles) {
   const double loads = (128.0 + static_cast<double>(columns) / t.ctas) * 128.0 / 140e3;
   const double mmas = columns * 2.0 / 1900.0;
   const int chunks = columns / 32;
-  const double epilogue = q.gated ? 0.7 + 0.53 * chunks : 0.6 + 0.3 * chunks;
+  const double epilogue = 0.6 + (q.gated ? 0.33 : 0.3) * chunks;
   const int k_tiles = (q.k + 127) / 128;
   const double steps = (k_tiles + t.split - 1) / t.split *
                        std::max(std::max(loads, mmas), t.sub == 2 ? 0.135 : 0.22);
@@ -276,7 +276,7 @@ int launch_product(const Product& q, void* stream) {
   }
   // 16-bit results leave through shared memory where the MMAs do not hide a store of 64 bytes a warp and
   // CTAs take several tiles: 8192 x 8192 x 64 takes 32.3 us against 38.6 with direct stores, k = 256 33.9
-  // against 39.6, gated 4096 x 8192 x 256 59.9 against 62.6; k = 1024 56.8 against 57.7; k = 2048 92.8
+  // against 39.6, gated 4096 x 8192 x 256 45.3 against 47.5; k = 1024 56.8 against 57.7; k = 2048 92.8
   // against 91.1. A CTA's only tile gains nothing: 300 x 4096 x 256 4.9 us against 4.7. The copies
   // write 16 bytes at a time, so rows of D must start, follow and end on multiples of eight.
   const long long walkers = sms / ctas;
