@@ -521,7 +521,8 @@ class Int8MoELayer:
     rows then up rows) with FP32 ``w13_scales`` ``[E, 2I]``, ``w2`` ``[E, H, I]`` with ``w2_scales``
     ``[E, H]``; ``quantize_int8_weights`` makes them. Every token is quantised with a scale of its
     own into the rows of its experts, the gate is applied in the first product's epilogue, and its
-    BF16 result is quantised again for the second.
+    BF16 result is quantised again for the second, whose FP32 rows are weighted and summed: an
+    expert's value may pass the largest FP16 number while the token's is ordinary.
 
     The experts' rows follow one another without padding and their offsets stay on the device
     (``nvfp4_moe_offsets``), so a forward is a fixed sequence of nine launches that reads nothing
@@ -579,9 +580,9 @@ class Int8MoELayer:
             h = int8.grouped_gemm(a, self.w13, a_scales, self.w13_scales, offsets, gated=True)
             a, a_scales = int8.quantize_tokens(h)
             y = int8.grouped_gemm(a, self.w2, a_scales, self.w2_scales, offsets,
-                                  out_dtype=torch.float16)
-            native.moe_combine(y.data_ptr(), row_of_pair.data_ptr(), weights.data_ptr(),
-                               out.data_ptr(), tokens, choices, self.hidden, stream)
+                                  out_dtype=torch.float32)
+            native.moe_combine_f32(y.data_ptr(), row_of_pair.data_ptr(), weights.data_ptr(),
+                                   out.data_ptr(), tokens, choices, self.hidden, stream)
         return out
 
 

@@ -155,6 +155,9 @@ _PROTOTYPES = {
     "nvfp4_moe_combine": (
         ctypes.c_int, [_P, _P, _P, _P, ctypes.c_int, ctypes.c_int, ctypes.c_int, _P],
     ),
+    "nvfp4_moe_combine_f32": (
+        ctypes.c_int, [_P, _P, _P, _P, ctypes.c_int, ctypes.c_int, ctypes.c_int, _P],
+    ),
     "nvfp4_moe_offsets": (ctypes.c_int, [_P, ctypes.c_int, _P, _P]),
     "nvfp4_moe_place_offsets": (
         ctypes.c_int, [_P, ctypes.c_int, ctypes.c_longlong, ctypes.c_int, ctypes.c_int, _P,
@@ -488,6 +491,12 @@ def moe_combine(y: int, row_of_pair: int, weights: int, out: int, tokens: int, c
                 hidden: int, stream: int) -> None:
     """``out[t] = sum_j weights[t, j] * y[row_of_pair[t * choices + j]]`` (FP16 rows, FP32 out)."""
     check(load().nvfp4_moe_combine(y, row_of_pair, weights, out, tokens, choices, hidden, stream))
+
+
+def moe_combine_f32(y: int, row_of_pair: int, weights: int, out: int, tokens: int, choices: int,
+                    hidden: int, stream: int) -> None:
+    """``moe_combine`` of FP32 rows."""
+    check(load().nvfp4_moe_combine_f32(y, row_of_pair, weights, out, tokens, choices, hidden, stream))
 
 
 def measure_mma_peak(device: int, iters: int = 4096) -> float:

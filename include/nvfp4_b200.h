@@ -355,6 +355,11 @@ int nvfp4_moe_place_routed(const void* ids, int ids_are_64bit, long long pairs, 
 int nvfp4_moe_combine(const void* y, const int* row_of_pair, const float* weights, float* out,
                       int tokens, int choices, int hidden, void* stream);
 
+/* The same of FP32 rows: what the INT8 path's second product writes, whose values may pass the
+ * largest FP16 number (65504). */
+int nvfp4_moe_combine_f32(const float* y, const int* row_of_pair, const float* weights, float* out,
+                          int tokens, int choices, int hidden, void* stream);
+
 /* Rows of experts that follow one another without padding: offsets[e] (device, `experts` + 1
  * ints) = pairs of the experts before e, from nvfp4_moe_count's counts, and the placement of every
  * pair in them (nvfp4_moe_place with the first rows on the device; `rows` at least the pairs).

@@ -853,3 +853,42 @@ def test_norm_codes_do_not_depend_on_how_rows_lie():
         single = int8.residual_norm(shifted[:, 1:], residual, post_weight=w, next_weight=w, quantize=True)
         for a, b, c in zip(many, few, single):
             assert torch.equal(a[:3], b) and torch.equal(a, c)
+
+
+def layer_by_experts(layer, x, ids, weights):
+    """(value, bound on the error) of the layer, an expert at a time. The codes and the gate's BF16 rows
+    are the operators' own, each tested above; the down projections and their sum are in 64 bits. A down
+    projection is an exact sum rounded to FP32 and two FP32 products, and the combine one fused
+    multiply-add for each choice: 3 + choices roundings of at most the sum of the terms' sizes."""
+    codes, scales = int8.quantize_tokens(x)
+    value, size = (torch.zeros(x.shape, dtype=torch.float64, device=DEV) for _ in range(2))
+    for e in range(layer.experts):
+        token, choice = torch.nonzero(ids == e, as_tuple=True)
+        if token.numel() == 0:
+            continue
+        h = int8.gemm(codes[token], layer.w13[e], scales[token], layer.w13_scales[e], gated=True)
+        q, t = int8.quantize_tokens(h)
+        y = (q.double() @ layer.w2[e].double().T) * t.double()[:, None] * layer.w2_scales[e].double()
+        term = y * weights[token, choice].double()[:, None]
+        value.index_add_(0, token, term)
+        size.index_add_(0, token, term.abs())
+    return value, (4 + ids.shape[1]) * U * size + 1e-40
+
+
+@pytest.mark.parametrize("tokens,hidden,inter,experts,choices,dtype", [
+    (1, 64, 32, 4, 2, torch.bfloat16), (5, 256, 96, 6, 3, torch.float32), (130, 512, 256, 8, 3, torch.float16),
+    (700, 256, 144, 5, 1, torch.bfloat16), (3000, 256, 96, 6, 2, torch.bfloat16)])
+@pytest.mark.parametrize("large", [1.0, 1e7])
+def test_int8_layer_keeps_every_row(tokens, hidden, inter, experts, choices, dtype, large):
+    """Each value by its own terms: rows of very different routing weights, weights of zero, and experts
+    whose down projections pass the largest FP16 number while the result is an ordinary FP32 one."""
+    layer, x, ids, weights = moe_case(tokens, hidden, inter, experts, choices, dtype)
+    layer.w2_scales = layer.w2_scales * large
+    g = rng_of(tokens + 1)
+    weights = weights * torch.exp(4 * torch.randn((tokens, 1), device=DEV, generator=g))
+    weights[::3, choices - 1] = 0.0
+    want, bound = layer_by_experts(layer, x, ids, weights)
+    got = layer.forward(x, ids, weights)
+    assert torch.isfinite(got).all()
+    assert ((got.double() - want).abs() <= bound).all()
+    int8.check_status(DEV)

@@ -180,3 +180,17 @@ def test_quantiser_reference_is_the_definition():
             np.testing.assert_array_equal(codes_, np.clip(np.rint(row / want), -127, 127))
         else:
             assert not codes_.any()
+
+
+def test_combine_of_fp32_rows_refuses_before_cuda(library):
+    def combine(y=16, rows=16, weights=16, out=16, tokens=4, choices=2, hidden=16):
+        return library.nvfp4_moe_combine_f32(y, rows, weights, out, tokens, choices, hidden, None)
+
+    for name in ("y", "rows", "weights", "out"):
+        assert combine(**{name: None}) == native.E_INVALID_ARGUMENT
+    assert combine(tokens=-1) == native.E_UNSUPPORTED_SHAPE
+    assert combine(choices=0) == native.E_UNSUPPORTED_SHAPE
+    assert combine(hidden=12) == native.E_UNSUPPORTED_SHAPE
+    assert combine(y=24) == native.E_MISALIGNED
+    assert combine(rows=18) == native.E_MISALIGNED
+    assert combine(tokens=0) == 0
