@@ -552,6 +552,7 @@ int nvfp4_residual_norm(const void* x, int x_kind, long long ldx, const void* re
                 hidden, kMaxHidden);
   }
   if (!(eps > 0.0) || !(eps < 1e30)) return fail(NVFP4_E_INVALID_ARGUMENT, "eps must be positive");
+  if (gate == nullptr && gates != 0) return fail(NVFP4_E_INVALID_ARGUMENT, "%d gates without a gate", gates);
   if (gate != nullptr && (gates < 1 || tokens % gates != 0)) {
     return fail(NVFP4_E_UNSUPPORTED_SHAPE, "%d tokens do not share %d gates evenly", tokens, gates);
   }

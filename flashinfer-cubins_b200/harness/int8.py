@@ -305,6 +305,8 @@ def residual_norm(x: torch.Tensor, residual: torch.Tensor | None = None, *,
     pgate, gates = None, 0
     if gate is not None:
         gates = gate.shape[0] if gate.dim() == 2 else 1
+        if gates == 0 or tokens % gates:  # the address of no rows is null, which is no gate
+            raise ValueError(f"{tokens} tokens do not share {gates} gates evenly")
         pgate = _vector(gate, (gates, hidden) if gate.dim() == 2 else row, "gate", index)
     _check_device(index)
     r, pr, ldr = None, None, 0

@@ -892,3 +892,14 @@ def test_int8_layer_keeps_every_row(tokens, hidden, inter, experts, choices, dty
     assert torch.isfinite(got).all()
     assert ((got.double() - want).abs() <= bound).all()
     int8.check_status(DEV)
+
+
+def test_norm_refuses_an_empty_gate():
+    """A gate of no rows is not the same as none: its address is null."""
+    x, w = torch.ones((6, 32), device=DEV), torch.ones(32, device=DEV)
+    for gates in (0, 4, 7):
+        with pytest.raises(ValueError):
+            int8.residual_norm(x, x, gate=torch.ones((gates, 32), device=DEV), next_weight=w)
+    with pytest.raises(ValueError):
+        int8.residual_norm(x[:0], x[:0], gate=torch.ones((0, 32), device=DEV), next_weight=w)
+    assert int8.residual_norm(x, x, gate=torch.ones((6, 32), device=DEV), next_weight=w)[0].shape == (6, 32)

@@ -194,3 +194,12 @@ def test_combine_of_fp32_rows_refuses_before_cuda(library):
     assert combine(y=24) == native.E_MISALIGNED
     assert combine(rows=18) == native.E_MISALIGNED
     assert combine(tokens=0) == 0
+
+
+def test_an_empty_gate_is_not_the_same_as_none(library):
+    """The address of a gate of no rows is null, which stands for no gate: it is refused, not left out."""
+    for gates in (0, 3):
+        with pytest.raises(ValueError):
+            int8.residual_norm(ones(4, 8), ones(4, 8), gate=ones(gates, 8), next_weight=ones(8))
+    assert library.nvfp4_residual_norm(16, 0, 8, 16, 0, 8, None, None, 2, 1.0, 16, 1e-6, 16, 8, 16, 0, 8, None,
+                                       4, 8, None) == native.E_INVALID_ARGUMENT
