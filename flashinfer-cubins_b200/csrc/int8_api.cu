@@ -556,12 +556,12 @@ int nvfp4_residual_norm(const void* x, int x_kind, long long ldx, const void* re
   if (gate != nullptr && (gates < 1 || tokens % gates != 0)) {
     return fail(NVFP4_E_UNSUPPORTED_SHAPE, "%d tokens do not share %d gates evenly", tokens, gates);
   }
+  if (tokens == 0) return 0;  // the addresses of empty tensors are null: the residual's says nothing here
   if (residual == nullptr &&
       (post_weight != nullptr || gate != nullptr || next_weight == nullptr || residual_scale != 1.0f)) {
     return fail(NVFP4_E_INVALID_ARGUMENT,
                 "without a residual there is only the norm of x: no post weight, gate or scale");
   }
-  if (tokens == 0) return 0;
   if (x == nullptr || (residual != nullptr && r == nullptr) ||
       (next_weight != nullptr && (y == nullptr || (y_kind == NVFP4_NORM_CODES && scales == nullptr)))) {
     return fail(NVFP4_E_INVALID_ARGUMENT, "null operand");

@@ -287,8 +287,9 @@ def residual_norm(x: torch.Tensor, residual: torch.Tensor | None = None, *,
             raise ValueError(f"residual: expected {tuple(shape)} beside the first operand, got "
                              f"{residual.dtype} {tuple(residual.shape)} on {residual.device}")
         pres, ldres = residual.data_ptr(), _rows(residual, shape, "residual")
-    elif residual_out is not None:
-        raise ValueError("residual_out without a residual")
+    elif residual_out is not None or post_weight is not None or gate is not None or residual_scale != 1.0:
+        raise ValueError("without a residual there is only the norm of x: no post_weight, gate, residual_scale "
+                         "or residual_out")
     if next_weight is None and (residual is None or quantize or out_dtype is not None):
         raise ValueError("next_weight is missing: there is nothing to norm, quantise or return")
     if quantize and out_dtype is not None:

@@ -903,3 +903,24 @@ def test_norm_refuses_an_empty_gate():
     with pytest.raises(ValueError):
         int8.residual_norm(x[:0], x[:0], gate=torch.ones((0, 32), device=DEV), next_weight=w)
     assert int8.residual_norm(x, x, gate=torch.ones((6, 32), device=DEV), next_weight=w)[0].shape == (6, 32)
+
+
+def test_norms_and_block_of_no_tokens():
+    """A batch without tokens (an expert-parallel rank may have none) gives empty results in every form."""
+    from harness import moe
+
+    x, w = torch.ones((0, 256), device=DEV), torch.ones(256, device=DEV)
+    for residual in (x, x.bfloat16(), x.half()):
+        for post in (None, w):
+            for gate in (None, w, w.view(1, 256)):
+                call = dict(post_weight=post, gate=gate, residual_scale=0.5)
+                r, y, s = int8.residual_norm(x, residual, **call)
+                assert r.shape == (0, 256) and r.dtype == residual.dtype and y is None and s is None
+                r, y, s = int8.residual_norm(x, residual, next_weight=w, **call)
+                assert r.shape == y.shape == (0, 256) and y.dtype == residual.dtype and s is None
+                r, y, s = int8.residual_norm(x, residual, next_weight=w, quantize=True, **call)
+                assert r.shape == y.shape == (0, 256) and y.dtype == torch.int8 and s.shape == (0,)
+    layer, x, ids, weights = moe_case(4, 256, 96, 6, 2)
+    block = moe.MoEBlock(layer, w, w, w.view(1, 256), 0.7)
+    got, normed = block.forward(x[:0], lambda n: (ids[:0], weights[:0]), next_weight=w)
+    assert got.shape == normed.shape == (0, 256)

@@ -203,3 +203,17 @@ def test_an_empty_gate_is_not_the_same_as_none(library):
             int8.residual_norm(ones(4, 8), ones(4, 8), gate=ones(gates, 8), next_weight=ones(8))
     assert library.nvfp4_residual_norm(16, 0, 8, 16, 0, 8, None, None, 2, 1.0, 16, 1e-6, 16, 8, 16, 0, 8, None,
                                        4, 8, None) == native.E_INVALID_ARGUMENT
+
+
+def test_norms_of_no_tokens_are_no_error(library):
+    """The address of an empty tensor is null: without tokens a null residual stands for nothing, and what
+    does not fit together is refused by the function for any number of tokens."""
+    for post, gate, gates, scale in ((16, None, 0, 1.0), (None, 16, 1, 1.0), (None, None, 0, 0.5)):
+        for weight in (16, None):
+            assert library.nvfp4_residual_norm(None, 0, 8, None, 0, 8, post, gate, gates, scale, weight, 1e-6,
+                                               None, 8, None, 0, 8, None, 0, 8, None) == 0
+    w = ones(8)
+    for wrong in (dict(post_weight=w), dict(gate=w), dict(residual_scale=0.5), dict(residual_out=ones(0, 8))):
+        for tokens in (0, 4):
+            with pytest.raises(ValueError):
+                int8.residual_norm(ones(tokens, 8), next_weight=w, **wrong)
