@@ -45,6 +45,8 @@ bool is_in_kind(int kind) {
 // Sums of k products of two codes of -128..127 stay below 2^31 up to here.
 constexpr int kMaxDepth = 131071;
 constexpr int kMaxHidden = 32768;
+// 1 / sqrt(eps) is 3.2e38, below FP32's largest number: a row's factor is finite, and a zero row zero.
+constexpr double kMinEps = 1e-77;
 // Rows of A, and of B: sums of a tile's rows stay within 32 bits.
 constexpr int kMaxRows = 1 << 30;
 
@@ -551,7 +553,9 @@ int nvfp4_residual_norm(const void* x, int x_kind, long long ldx, const void* re
     return fail(NVFP4_E_UNSUPPORTED_SHAPE, "unsupported rows: %d of %d (at most %d wide)", tokens,
                 hidden, kMaxHidden);
   }
-  if (!(eps > 0.0) || !(eps < 1e30)) return fail(NVFP4_E_INVALID_ARGUMENT, "eps must be positive");
+  if (!(eps >= kMinEps) || !(eps < 1e30)) {
+    return fail(NVFP4_E_INVALID_ARGUMENT, "eps must be at least %g and below 1e30", kMinEps);
+  }
   if (gate == nullptr && gates != 0) return fail(NVFP4_E_INVALID_ARGUMENT, "%d gates without a gate", gates);
   if (gate != nullptr && (gates < 1 || tokens % gates != 0)) {
     return fail(NVFP4_E_UNSUPPORTED_SHAPE, "%d tokens do not share %d gates evenly", tokens, gates);

@@ -263,8 +263,8 @@ def residual_norm(x: torch.Tensor, residual: torch.Tensor | None = None, *,
     Returns ``(r, y, scales)``: ``r`` in the residual's type, ``y`` (of the unrounded ``r``) in
     ``out_dtype`` (default: the residual's type) or, with ``quantize``, as INT8 codes with their
     ``scales``; what is not made is None. ``gate`` is ``[hidden]`` or ``[gates, hidden]``, each row
-    for ``tokens / gates`` consecutive tokens. Weights and gate are FP32, ``eps`` is above zero. Without a residual only
-    ``y = x / rms(x) * next_weight`` is made. ``residual_out`` (may be ``residual`` itself) and ``out``
+    for ``tokens / gates`` consecutive tokens. Weights and gate are FP32, ``eps`` is at least 1e-77. Without a residual
+    only ``y = x / rms(x) * next_weight`` is made. ``residual_out`` (may be ``residual`` itself) and ``out``
     (``y``, or codes and scales) are tensors to write to."""
     index, device = x.get_device(), x.device
     if torch.is_grad_enabled() and (

@@ -413,7 +413,8 @@ int nvfp4_int8_quantize(const void* x, int x_kind, long long ldx, const int* sou
  *   p = post_weight ? x / rms(x) * post_weight : x        (the norm after the block)
  *   r = residual_scale * residual + (gate ? gate * p : p) (r in the residual's type)
  *   y = r / rms(r) * next_weight                          (the norm before the next; of the FP32 r)
- * with rms(v) = sqrt(mean(v^2) + eps). Weights and gate are FP32; gate [gates][hidden], each row for
+ * with rms(v) = sqrt(mean(v^2) + eps), eps at least 1e-77 (a zero row's factor is finite then).
+ * Weights and gate are FP32; gate [gates][hidden], each row for
  * tokens / gates consecutive tokens (gates 0 with a null gate). next_weight may be null (no y);
  * residual may be null, then only y = x / rms(x) * next_weight is made. y_kind: NVFP4_IN_* or
  * NVFP4_NORM_CODES, INT8 codes and `scales` as nvfp4_int8_quantize makes them of the FP32 y. r may be

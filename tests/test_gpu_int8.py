@@ -924,3 +924,20 @@ def test_norms_and_block_of_no_tokens():
     block = moe.MoEBlock(layer, w, w, w.view(1, 256), 0.7)
     got, normed = block.forward(x[:0], lambda n: (ids[:0], weights[:0]), next_weight=w)
     assert got.shape == normed.shape == (0, 256)
+
+
+@pytest.mark.parametrize("hidden", [40, 41, 2048])
+def test_norm_with_the_smallest_eps(hidden):
+    """Zero rows give zeros with every eps that is taken, rows of subnormals their value."""
+    x = torch.zeros((3, hidden), device=DEV)
+    x[1] = 1e-40
+    w = torch.ones(hidden, device=DEV)
+    want = x.double() / (x.double().square().mean(1, keepdim=True) + 1e-77).sqrt()
+    _, y, _ = int8.residual_norm(x, next_weight=w, eps=1e-77)
+    assert (y[0] == 0).all() and (y[2] == 0).all()
+    torch.testing.assert_close(y.double(), want, rtol=4 * U, atol=0)
+    _, q, s = int8.residual_norm(x, next_weight=w, eps=1e-77, quantize=True)
+    assert not q[0].any() and (q[1] == 127).all() and s[0] == 0 and s[2] == 0
+    for eps in (0.9e-77, 1e-100, 5e-324, 0.0, -1e-6):
+        with pytest.raises(ValueError):
+            int8.residual_norm(x, next_weight=w, eps=eps)

@@ -217,3 +217,15 @@ def test_norms_of_no_tokens_are_no_error(library):
         for tokens in (0, 4):
             with pytest.raises(ValueError):
                 int8.residual_norm(ones(tokens, 8), next_weight=w, **wrong)
+
+
+def test_an_eps_whose_root_has_no_fp32_reciprocal_is_refused(library):
+    """1 / sqrt(eps) beyond FP32 would make NaN of a zero row."""
+    def norm(eps):
+        return library.nvfp4_residual_norm(None, 0, 8, None, 0, 8, None, None, 0, 1.0, 16, eps, None, 8, None, 0,
+                                           8, None, 0, 8, None)
+
+    for eps in (1e-77, 1e-6, 1e29):
+        assert norm(eps) == 0
+    for eps in (0.99e-77, 1e-100, 5e-324, 1e30, float("inf")):
+        assert norm(eps) == native.E_INVALID_ARGUMENT
