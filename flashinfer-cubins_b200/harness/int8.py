@@ -11,8 +11,8 @@ Each call is one launch, asynchronous on the current stream of its tensors' devi
 for the launch where it is not), without a workspace, a plan or anything kept for the next call: it
 can be captured in a CUDA graph and called from several threads and streams at once. A call with
 wrong operands raises ``ValueError`` before anything is launched, one on a device that is not
-compute capability 10.0 ``RuntimeError``. There is no backward: operands that require a gradient
-are refused while gradients are recorded.
+compute capability 10.0 ``RuntimeError``. There are no derivatives: operands that require a gradient
+are refused while gradients are recorded, operands with a tangent of forward differentiation always.
 
 Codes are ``torch.int8`` ``[rows, k]`` whose rows start 16-byte aligned and a multiple of 16 bytes
 apart, which is what ``quantize_tokens`` and ``residual_norm`` return for every ``k`` (a view of
@@ -24,6 +24,7 @@ and contiguous. Weights are quantised by the same function, a scale for each out
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from . import native
 
@@ -69,6 +70,13 @@ def _launch(index: int, entry: str, *arguments) -> None:
 
 def _refuse_gradients() -> None:
     raise ValueError("the INT8 operators have no backward; call them under torch.no_grad()")
+
+
+def refuse_tangents(*tensors: torch.Tensor | None) -> None:
+    """Refuse operands of forward differentiation (which no_grad does not switch off)."""
+    if forward_ad._current_level >= 0 and any(
+            t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise ValueError("the INT8 operators have no derivatives: an operand has a tangent")
 
 
 def check_status(device: torch.device | str | int | None = None) -> None:
@@ -144,6 +152,7 @@ def gemm(a: torch.Tensor, b: torch.Tensor, a_scales: torch.Tensor, b_scales: tor
                                     or (bias is not None and bias.requires_grad)
                                     or (out is not None and out.requires_grad)):
         _refuse_gradients()
+    refuse_tangents(a_scales, b_scales, bias, out)
     lda, ldb = _codes(a, 2, "a", index), _codes(b, 2, "b", index)
     (m, k), (width, depth) = a.shape, b.shape
     if depth != k:
@@ -179,6 +188,7 @@ def grouped_gemm(a: torch.Tensor, b: torch.Tensor, a_scales: torch.Tensor, b_sca
     if torch.is_grad_enabled() and (a_scales.requires_grad or b_scales.requires_grad
                                     or (out is not None and out.requires_grad)):
         _refuse_gradients()
+    refuse_tangents(a_scales, b_scales, out)
     lda, ldb = _codes(a, 2, "a", index), _codes(b, 3, "b", index)
     (rows, k), (experts, width, depth) = a.shape, b.shape
     if depth != k:
@@ -217,6 +227,7 @@ def quantize_tokens(x: torch.Tensor, *, rows: torch.Tensor | None = None,
     index = x.get_device()
     if torch.is_grad_enabled() and (x.requires_grad or (out is not None and out[1].requires_grad)):
         _refuse_gradients()
+    refuse_tangents(x, None if out is None else out[1])
     kind = IN_KINDS.get(x.dtype)
     if x.dim() != 2 or kind is None:
         raise ValueError(f"x: expected 2-d FP32, BF16 or FP16, got {x.dtype} {tuple(x.shape)}")
@@ -274,6 +285,8 @@ def residual_norm(x: torch.Tensor, residual: torch.Tensor | None = None, *,
             or (residual_out is not None and residual_out.requires_grad)
             or (out is not None and any(t.requires_grad for t in (out if quantize else (out,))))):
         _refuse_gradients()
+    refuse_tangents(x, residual, post_weight, gate, next_weight, residual_out,
+                    out[1] if quantize and out is not None else out)
     x_kind = IN_KINDS.get(x.dtype)
     if x.dim() != 2 or x_kind is None:
         raise ValueError(f"x: expected 2-d FP32, BF16 or FP16, got {x.dtype} {tuple(x.shape)}")

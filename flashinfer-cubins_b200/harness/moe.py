@@ -557,6 +557,7 @@ class Int8MoELayer:
             raise ValueError("operands must be on the layer's device")
         if torch.is_grad_enabled() and (x.requires_grad or topk_weights.requires_grad):
             raise ValueError("the INT8 layer has no backward; call it under torch.no_grad()")
+        int8.refuse_tangents(x, topk_weights)
         pairs = tokens * choices
         out = torch.empty((tokens, self.hidden), dtype=torch.float32, device=self.device)
         if pairs == 0:

@@ -941,3 +941,16 @@ def test_norm_with_the_smallest_eps(hidden):
     for eps in (0.9e-77, 1e-100, 5e-324, 0.0, -1e-6):
         with pytest.raises(ValueError):
             int8.residual_norm(x, next_weight=w, eps=eps)
+
+
+def test_layer_refuses_forward_gradients():
+    from torch.autograd import forward_ad
+
+    layer, x, ids, weights = moe_case(4, 256, 96, 6, 2)
+    want = layer.forward(x, ids, weights)
+    with forward_ad.dual_level():
+        for call in (lambda: layer.forward(forward_ad.make_dual(x, torch.ones_like(x)), ids, weights),
+                     lambda: layer.forward(x, ids, forward_ad.make_dual(weights, torch.ones_like(weights)))):
+            with pytest.raises(ValueError):
+                call()
+        assert torch.equal(layer.forward(x, ids, weights), want)

@@ -229,3 +229,44 @@ def test_an_eps_whose_root_has_no_fp32_reciprocal_is_refused(library):
         assert norm(eps) == 0
     for eps in (0.99e-77, 1e-100, 5e-324, 1e30, float("inf")):
         assert norm(eps) == native.E_INVALID_ARGUMENT
+
+
+def test_functions_refuse_forward_gradients():
+    """A tangent would be dropped without a word; operands without one pass the check inside a level of
+    forward differentiation, under no_grad too (which does not switch it off)."""
+    from torch.autograd import forward_ad
+
+    a, b, sa, sb = codes(3, 32), codes(8, 32), ones(3), ones(8)
+    experts, offsets = codes(2, 8, 32), torch.zeros(3, dtype=torch.int32)
+    x, w = ones(4, 16), ones(16)
+    with forward_ad.dual_level():
+        def dual(t):
+            return forward_ad.make_dual(t.clone(), torch.ones_like(t))
+
+        calls = (
+            lambda: int8.gemm(a, b, dual(sa), sb),
+            lambda: int8.gemm(a, b, sa, dual(sb)),
+            lambda: int8.gemm(a, b, sa, sb, bias=dual(ones(8))),
+            lambda: int8.gemm(a, b, sa, sb, out_dtype=torch.float32, out=dual(ones(3, 8))),
+            lambda: int8.grouped_gemm(a, experts, dual(sa), ones(2, 8), offsets),
+            lambda: int8.grouped_gemm(a, experts, sa, dual(ones(2, 8)), offsets),
+            lambda: int8.quantize_tokens(dual(x)),
+            lambda: int8.quantize_tokens(x, out=(codes(4, 16), dual(ones(4)))),
+            lambda: int8.residual_norm(dual(x), next_weight=w),
+            lambda: int8.residual_norm(x, dual(x), next_weight=w),
+            lambda: int8.residual_norm(x, x, post_weight=dual(w), next_weight=w),
+            lambda: int8.residual_norm(x, x, gate=dual(w), next_weight=w),
+            lambda: int8.residual_norm(x, next_weight=dual(w)),
+            lambda: int8.residual_norm(x, x, next_weight=w, residual_out=dual(x)),
+            lambda: int8.residual_norm(x, next_weight=w, out=dual(x)),
+            lambda: int8.residual_norm(x, next_weight=w, quantize=True, out=(codes(4, 16), dual(ones(4)))),
+        )
+        for call in calls:
+            with pytest.raises(ValueError):
+                call()
+            with torch.no_grad(), pytest.raises(ValueError):
+                call()
+        for call in (lambda: int8.gemm(a, b, sa, sb), lambda: int8.quantize_tokens(x),
+                     lambda: int8.residual_norm(x, x, next_weight=w)):
+            with pytest.raises(RuntimeError):       # no device
+                call()
