@@ -47,7 +47,8 @@ constexpr int kMaxDepth = 131071;
 constexpr int kMaxHidden = 32768;
 // 1 / sqrt(eps) is 3.2e38, below FP32's largest number: a row's factor is finite, and a zero row zero.
 constexpr double kMinEps = 1e-77;
-// Rows of A, and of B: sums of a tile's rows stay within 32 bits.
+// Rows of any operand, and elements of a row of the quantiser: a count and a tile, a CTA's rows or a
+// step of its threads together stay within 32 bits.
 constexpr int kMaxRows = 1 << 30;
 
 // One product, dense (offsets null, one expert) or grouped.
@@ -507,8 +508,9 @@ int nvfp4_int8_status(void* stream, int* status) {
 int nvfp4_int8_quantize(const void* x, int x_kind, long long ldx, const int* source_rows, int rows,
                         int tokens, int k, void* q, long long ldq, float* scales, void* stream) {
   if (!is_in_kind(x_kind)) return fail(NVFP4_E_INVALID_ARGUMENT, "unknown input kind %d", x_kind);
-  if (rows < 0 || tokens < 0 || k < 1) {
-    return fail(NVFP4_E_UNSUPPORTED_SHAPE, "unsupported tensor: %d rows of %d, k=%d", rows, tokens, k);
+  if (rows < 0 || rows > kMaxRows || tokens < 0 || tokens > kMaxRows || k < 1 || k > kMaxRows) {
+    return fail(NVFP4_E_UNSUPPORTED_SHAPE, "unsupported tensor: %d rows of %d, k=%d (at most %d each)", rows,
+                tokens, k, kMaxRows);
   }
   if (rows == 0) return 0;
   if (source_rows == nullptr && rows != tokens) {
@@ -549,7 +551,7 @@ int nvfp4_residual_norm(const void* x, int x_kind, long long ldx, const void* re
     return fail(NVFP4_E_INVALID_ARGUMENT, "unknown type: x %d, residual %d, y %d", x_kind,
                 residual_kind, y_kind);
   }
-  if (tokens < 0 || hidden < 1 || hidden > kMaxHidden) {
+  if (tokens < 0 || tokens > kMaxRows || hidden < 1 || hidden > kMaxHidden) {
     return fail(NVFP4_E_UNSUPPORTED_SHAPE, "unsupported rows: %d of %d (at most %d wide)", tokens,
                 hidden, kMaxHidden);
   }

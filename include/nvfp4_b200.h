@@ -405,7 +405,8 @@ int nvfp4_int8_status(void* stream, int* status);
  * quotients correctly rounded. A zero row has scale 0; a row with an infinity or a NaN has that as
  * its scale and zero codes, so that its products are NaN. With source_rows (device, `rows` ints)
  * row r is row source_rows[r] of the `tokens` rows of x; where that is negative or beyond them the
- * row's codes and scale are left as they were. Without, rows = tokens. */
+ * row's codes and scale are left as they were. Without, rows = tokens. rows, tokens and k are at most
+ * 2^30. */
 int nvfp4_int8_quantize(const void* x, int x_kind, long long ldx, const int* source_rows, int rows,
                         int tokens, int k, void* q, long long ldq, float* scales, void* stream);
 
@@ -418,7 +419,7 @@ int nvfp4_int8_quantize(const void* x, int x_kind, long long ldx, const int* sou
  * tokens / gates consecutive tokens (gates 0 with a null gate). next_weight may be null (no y);
  * residual may be null, then only y = x / rms(x) * next_weight is made. y_kind: NVFP4_IN_* or
  * NVFP4_NORM_CODES, INT8 codes and `scales` as nvfp4_int8_quantize makes them of the FP32 y. r may be
- * the residual itself. */
+ * the residual itself. At most 2^30 tokens. */
 #define NVFP4_NORM_CODES (-1)
 int nvfp4_residual_norm(const void* x, int x_kind, long long ldx, const void* residual,
                         int residual_kind, long long ldres, const float* post_weight,

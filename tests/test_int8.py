@@ -270,3 +270,18 @@ def test_functions_refuse_forward_gradients():
                      lambda: int8.residual_norm(x, x, next_weight=w)):
             with pytest.raises(RuntimeError):       # no device
                 call()
+
+
+def test_counts_beyond_the_kernels_32_bits_are_refused(library):
+    """An index that runs a step past 2^31 - 1 would turn negative."""
+    most, over = 1 << 30, (1 << 30) + 1
+
+    def quantize(source=None, rows=4, tokens=4, k=8):
+        return library.nvfp4_int8_quantize(16, 0, 1 << 31, source, rows, tokens, k, 16, 1 << 31, 16, None)
+
+    for wrong in (dict(k=over), dict(k=(1 << 31) - 1), dict(rows=over, tokens=over), dict(source=16, rows=over),
+                  dict(source=16, tokens=over)):
+        assert quantize(**wrong) == native.E_UNSUPPORTED_SHAPE
+    assert quantize(rows=0, tokens=0, k=most) == 0
+    assert library.nvfp4_residual_norm(16, 0, 8, 16, 0, 8, None, None, 0, 1.0, 16, 1e-6, 16, 8, 16, 0, 8, None,
+                                       over, 8, None) == native.E_UNSUPPORTED_SHAPE
