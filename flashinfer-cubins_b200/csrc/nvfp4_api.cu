@@ -1827,11 +1827,11 @@ static int moe_place_common(const void* ids, int ids_are_64bit, long long pairs,
   if (ids_are_64bit) {
     moe_place_kernel<long long><<<blocks, threads, 0, s>>>(static_cast<const long long*>(ids), pairs,
                                                            choices, experts, starts,
-                                                           device_first_rows, cursors, row_of_pair,
+                                                           device_first_rows, rows, cursors, row_of_pair,
                                                            token_of_row);
   } else {
     moe_place_kernel<int><<<blocks, threads, 0, s>>>(static_cast<const int*>(ids), pairs, choices,
-                                                     experts, starts, device_first_rows, cursors,
+                                                     experts, starts, device_first_rows, rows, cursors,
                                                      row_of_pair, token_of_row);
   }
   CUDA_TRY(cudaGetLastError());

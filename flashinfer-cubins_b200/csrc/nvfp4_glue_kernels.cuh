@@ -253,7 +253,8 @@ quantize_nvfp4_kernel(const In* __restrict__ x, uint8_t* __restrict__ packed,
 //     combine, token_of_row[row] = i / choices for the gathering quantiser. Rows inside a
 //     block are handed out by an atomic counter: which pair gets which row differs from run
 //     to run, the result of the layer does not (every row is computed on its own).
-// Ids outside [0, experts) get no row (row_of_pair = -1).
+// Ids outside [0, experts) get no row (row_of_pair = -1), nor do pairs whose row would lie outside the
+// buffers: first rows that lie on the device cannot be checked before.
 constexpr int kMoeMaxExperts = 512;
 
 struct MoeStarts {
@@ -280,7 +281,7 @@ __global__ void moe_count_kernel(const Id* __restrict__ ids, long long pairs, in
 template <typename Id>
 __global__ void moe_place_kernel(const Id* __restrict__ ids, long long pairs, int choices,
                                  int experts, const __grid_constant__ MoeStarts starts,
-                                 const int* __restrict__ device_starts,
+                                 const int* __restrict__ device_starts, int rows,
                                  int* __restrict__ cursors, int* __restrict__ row_of_pair,
                                  int* __restrict__ token_of_row) {
   for (long long i = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x; i < pairs;
@@ -292,7 +293,11 @@ __global__ void moe_place_kernel(const Id* __restrict__ ids, long long pairs, in
       // was made on the device, from device memory.
       const int first = device_starts != nullptr ? __ldg(device_starts + e) : starts.first_row[e];
       row = first + atomicAdd(&cursors[e], 1);
-      token_of_row[row] = static_cast<int>(i / choices);
+      if (row >= 0 && row < rows) {
+        token_of_row[row] = static_cast<int>(i / choices);
+      } else {  // first rows that are not these ids'
+        row = -1;
+      }
     }
     row_of_pair[i] = row;
   }

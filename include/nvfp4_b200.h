@@ -306,7 +306,8 @@ int nvfp4_quantize_gather(const void* x, int x_kind, void* packed, void* scales,
  *     padded to 128) every pair gets a row of its expert's block: row_of_pair[i] (device,
  *     `pairs` ints) and token_of_row[row] = i / choices (device, `rows` ints, -1 for the rows
  *     that hold no pair). `cursors` is device scratch of `experts` ints. Which pair gets which
- *     row of a block may differ from run to run; the layer's result does not depend on it.
+ *     row of a block may differ from run to run; the layer's result does not depend on it. A pair
+ *     whose row would lie outside [0, rows) gets none (-1).
  * The reference routes on the host (harness/workloads/moe.py:1-33 describes its FP8 layer's
  * stages); no counterpart on this path. */
 int nvfp4_moe_count(const void* ids, int ids_are_64bit, long long pairs, int experts, int* counts,

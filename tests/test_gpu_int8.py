@@ -954,3 +954,27 @@ def test_layer_refuses_forward_gradients():
             with pytest.raises(ValueError):
                 call()
         assert torch.equal(layer.forward(x, ids, weights), want)
+
+
+@pytest.mark.parametrize("offsets", [[5, 6, 7, 7, 8, 8], [0, 0, 0, 0, -2, 0], [(1 << 31) - 1, 0, 0, -(1 << 31), 3, 3],
+                                     [8, 8, 8, 8, 8, 8]])
+def test_placement_never_reaches_outside_the_rows(offsets):
+    """Offsets that are not those of the ids: pairs whose row would lie outside the buffers have none, and
+    nothing beside the rows is written."""
+    ids = torch.tensor([[3, 0], [3, 9], [-1, 0], [3, 1]], dtype=torch.int64, device=DEV)
+    buffer = torch.full((24,), -9, dtype=torch.int32, device=DEV)
+    token_of_row = buffer[8:16]
+    row_of_pair, cursors = torch.full((8,), -9, dtype=torch.int32, device=DEV), torch.zeros(5, dtype=torch.int32, device=DEV)
+    starts = torch.tensor(offsets, dtype=torch.int32, device=DEV)
+    native.moe_place_offsets(ids.data_ptr(), True, 8, 2, 5, starts.data_ptr(), 8, cursors.data_ptr(),
+                             row_of_pair.data_ptr(), token_of_row.data_ptr(), torch.cuda.current_stream().cuda_stream)
+    assert (buffer[:8] == -9).all() and (buffer[16:] == -9).all()
+    # Every expert's pairs have its rows from its offset on, in any order, as far as they lie inside.
+    rows = row_of_pair.tolist()
+    for e, pairs in ((0, (1, 5)), (1, (7,)), (3, (0, 2, 6))):
+        want = [offsets[e] + i if 0 <= offsets[e] + i < 8 else -1 for i in range(len(pairs))]
+        assert sorted(rows[i] for i in pairs) == sorted(want)
+    assert rows[3] == rows[4] == -1
+    tokens = token_of_row.tolist()
+    for row, token in enumerate(tokens):
+        assert token in ([i // 2 for i in range(8) if rows[i] == row] or [-1])
