@@ -103,10 +103,6 @@ TileKernel tile_kernel(int ctas, int sub, bool gated) {
   return gated ? int8_tile_kernel<2, 2, true> : int8_tile_kernel<2, 2, false>;
 }
 
-// What a block can have of shared memory, less the kernels' static share (barriers and the epilogue's
-// scales, 4.4 KB) and the slack that aligns the stages to 1,024 bytes.
-constexpr int kSharedLimit = 232448 - 5 * 1024;
-
 // Codes (128-byte swizzle), or with `output` 16-bit elements as they lie.
 int encode(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims,
            const cuuint64_t* strides, const cuuint32_t* box, bool output = false) {
@@ -150,10 +146,10 @@ int cluster_slots(int split, int sms) {
   cudaLaunchConfig_t config{};
   config.gridDim = dim3(static_cast<unsigned int>(split));
   config.blockDim = dim3(int8_threads(32));
-  config.dynamicSmemBytes = kSharedLimit;
+  config.dynamicSmemBytes = kInt8SharedLimit;
   config.attrs = attribute;
   config.numAttrs = 1;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSharedLimit) != cudaSuccess ||
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kInt8SharedLimit) != cudaSuccess ||
       cudaOccupancyMaxActiveClusters(&count, kernel, &config) != cudaSuccess || count < 1) {
     cudaGetLastError();
     return sms / split * 3 / 4;
@@ -283,8 +279,10 @@ int launch_product(const Product& q, void* stream) {
   // against 91.1. A CTA's only tile gains nothing: 300 x 4096 x 256 4.9 us against 4.7. The copies
   // write 16 bytes at a time, so rows of D must start, follow and end on multiples of eight.
   const long long walkers = sms / ctas;
-  p.staged = q.out_kind != NVFP4_OUT_F32 && q.k <= 1024 && split == 1 && tiles > walkers && q.n % 8 == 0 &&
-             q.ldd % 8 == 0 && aligned(q.d, 16);
+  const bool may_stage = q.out_kind != NVFP4_OUT_F32 && q.k <= 1024 && split == 1 && tiles > walkers &&
+                         q.n % 8 == 0 && q.ldd % 8 == 0 && aligned(q.d, 16);
+  const Int8Ring ring = int8_ring(ctas, tile_tokens, tiling.sub, q.k, q.experts, may_stage);
+  p.staged = ring.staged;
   if (p.staged) {
     const cuuint64_t dims[2] = {static_cast<cuuint64_t>(q.n), static_cast<cuuint64_t>(q.rows)};
     const cuuint64_t strides[1] = {static_cast<cuuint64_t>(q.ldd) * 2};
@@ -306,15 +304,11 @@ int launch_product(const Product& q, void* stream) {
   p.split = split;
   p.tmem_columns = 32;
   while (p.tmem_columns < (split > 1 ? 1 : 2) * tile_tokens) p.tmem_columns *= 2;
-  const int stage_bytes = tiling.sub * 128 * (128 + tile_tokens / ctas);
-  const int tables = 8 * (q.experts + 1) +
-                     (p.staged ? 4 * int8_parts(tile_tokens) * static_cast<int>(kInt8StagedBytes) : 0);
-  p.stages = std::min(kInt8MaxStages, (kSharedLimit - 1024 - tables) / stage_bytes);
-  const size_t shared = static_cast<size_t>(p.stages) * stage_bytes + 1024 + tables;
+  p.stages = ring.stages;
 
   const TileKernel kernel = tile_kernel(ctas, tiling.sub, q.gated);
   CUDA_TRY(cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                                cudaFuncAttributeMaxDynamicSharedMemorySize, kSharedLimit));
+                                cudaFuncAttributeMaxDynamicSharedMemorySize, kInt8SharedLimit));
   const int group = split > 1 ? split : ctas;
   // A split tile is a cluster's only one; otherwise a CTA (or pair) on every SM walks the tiles.
   const long long groups = split > 1 ? tiles : std::min(tiles, walkers);
@@ -328,7 +322,7 @@ int launch_product(const Product& q, void* stream) {
   cudaLaunchConfig_t config{};
   config.gridDim = dim3(static_cast<unsigned int>(groups * group));
   config.blockDim = dim3(int8_threads(tile_tokens));
-  config.dynamicSmemBytes = shared;
+  config.dynamicSmemBytes = static_cast<size_t>(ring.bytes);
   config.stream = static_cast<cudaStream_t>(stream);
   config.attrs = attribute;
   config.numAttrs = group > 1 ? 2 : 1;

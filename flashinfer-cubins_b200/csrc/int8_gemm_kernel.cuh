@@ -27,20 +27,10 @@
 #include <cuda.h>
 
 #include "int8_kernels.cuh"
+#include "int8_ring.h"
 
 namespace nvfp4 {
 
-// Epilogue warps: four (one for each quarter of tensor memory's lanes) for every 32 tokens of a tile,
-// up to sixteen. A tile of 256 tokens then leaves in two rounds of 32 tokens a warp; with four warps
-// the epilogue took longer than the MMAs of 4096 k (gated 1000 x 14336 x 4096: 153 us, now 84), and
-// warps without work only poll.
-constexpr int kInt8MaxParts = 4;
-constexpr int int8_parts(int tile_tokens) {
-  return tile_tokens / 32 < kInt8MaxParts ? tile_tokens / 32 : kInt8MaxParts;
-}
-constexpr int int8_threads(int tile_tokens) { return 64 + 128 * int8_parts(tile_tokens); }
-constexpr int kInt8MaxStages = 12;
-constexpr int kInt8MaxExperts = 1024;
 // Token tiles that are walked together, channel tile by channel tile, for the L2 cache: 8192^3 takes 348,
 // 340 and 333 us with bands of 4, 8 and 16, 32 experts of 4096 rows, gated 2048 x 7168, 183, 184 and 187.
 constexpr int kInt8Band = 8;
@@ -194,8 +184,6 @@ __device__ __forceinline__ void tma_store_rows(const void* map, uint32_t src, in
 
 // 32 tokens of a warp's channels through its 2 KB of shared memory, a 16-bit value at a time: the
 // addresses are constants apart, where a store to D needs one of its own.
-constexpr uint32_t kInt8StagedBytes = 2048;
-
 template <typename T, int COLUMNS>
 __device__ __forceinline__ void stage_columns(uint32_t to, uint32_t step, const float (&v)[COLUMNS]) {
 #pragma unroll

@@ -16,6 +16,7 @@ PACKAGE_ROOT = Path(__file__).resolve().parents[1]
 SOURCES = tuple(PACKAGE_ROOT / "csrc" / name for name in ("nvfp4_api.cu", "int8_api.cu"))
 HEADERS = (
     *sorted((PACKAGE_ROOT / "csrc").glob("*.cuh")),
+    PACKAGE_ROOT / "csrc" / "int8_ring.h",
     PACKAGE_ROOT / "csrc" / "nvfp4_host.h",
     PACKAGE_ROOT.parent / "include" / "nvfp4_b200.h",
 )

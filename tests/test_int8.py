@@ -285,3 +285,38 @@ def test_counts_beyond_the_kernels_32_bits_are_refused(library):
     assert quantize(rows=0, tokens=0, k=most) == 0
     assert library.nvfp4_residual_norm(16, 0, 8, 16, 0, 8, None, None, 0, 1.0, 16, 1e-6, 16, 8, 16, 0, 8, None,
                                        over, 8, None) == native.E_UNSUPPORTED_SHAPE
+
+
+def test_rings_of_products_let_loads_run_ahead(tmp_path):
+    """Every tile the products are cut into keeps two stages, so that loads and MMAs do not take turns,
+    unless its whole depth is one stage; with staging or without, and within a block's shared memory."""
+    import subprocess
+
+    header = native.LIBRARY_PATH.parents[1] / "csrc" / "int8_ring.h"
+    source = tmp_path / "rings.cpp"
+    source.write_text(f'#include "{header}"\n' + r"""
+#include <cstdio>
+#include <initializer_list>
+int main() {
+  for (int ctas = 1; ctas <= 2; ++ctas)
+    for (int tokens = 32 * ctas; tokens <= 256; tokens += 32)
+      for (int k : {1, 128, 129, 256, 257, 857, 1024, 131071})
+        for (int experts : {1, 2, 32, 1024})
+          for (int may = 0; may <= (k <= 1024); ++may) {
+            const int sub = ctas == 1 || tokens <= 128 ? 2 : 1;
+            const nvfp4::Int8Ring r = nvfp4::int8_ring(ctas, tokens, sub, k, experts, may);
+            std::printf("%d %d %d %d %d %d %d %d %d\n", ctas, tokens, sub, k, experts, may, r.stages, r.staged, r.bytes);
+          }
+}
+""")
+    program = tmp_path / "rings"
+    subprocess.run(["g++", "-std=c++17", "-o", str(program), str(source)], check=True)
+    lines = subprocess.run([str(program)], check=True, capture_output=True, text=True).stdout.splitlines()
+    assert len(lines) == 15 * 4 * (7 * 2 + 1)
+    for line in lines:
+        ctas, tokens, sub, k, experts, may, stages, staged, used = map(int, line.split())
+        assert stages >= (1 if k <= 128 * sub else 2), line
+        assert stages <= 12 and used <= 232448 - 5 * 1024 and (may or not staged), line
+        stage = sub * 128 * (128 + tokens // ctas)
+        warps = 4 * min(tokens // 32, 4)
+        assert used == 1024 + stages * stage + 8 * (experts + 1) + staged * warps * 2048, line
