@@ -978,3 +978,66 @@ def test_placement_never_reaches_outside_the_rows(offsets):
     tokens = token_of_row.tolist()
     for row, token in enumerate(tokens):
         assert token in ([i // 2 for i in range(8) if rows[i] == row] or [-1])
+
+
+@pytest.mark.parametrize("m,n,k", [(3, 96, 6832), (277, 256, 5136), (313, 416, 1500), (33, 130, 2049), (842, 40, 9008),
+                                   (120, 24, 640), (60, 300, 4097), (2297, 585, 300)])
+@pytest.mark.parametrize("gated", [False, True])
+def test_groups_of_few_tiles_with_weights_of_their_own(m, n, k, gated):
+    """Every expert's weights and scales differ: a product with another expert's fails at any depth."""
+    g = rng_of(m * n + k)
+    width = 2 * n if gated else n
+    a, b = make_codes(g, m, k), make_codes(g, 4, width, k)
+    sa = 0.5 + torch.rand(m, device=DEV, generator=g)
+    sb = (0.5 + torch.rand((4, width), device=DEV, generator=g)) * (2e-4 / k ** 0.5)
+    edges = [0, m // 3, m // 3, m - 1, m]
+    offsets = torch.tensor(edges, dtype=torch.int32, device=DEV)
+    for dtype in DTYPES:
+        out, check = guarded(m, n, dtype)
+        int8.grouped_gemm(a, b, sa, sb, offsets, gated=gated, out_dtype=dtype, out=out)
+        check()
+        for e, (lo, hi) in enumerate(zip(edges, edges[1:])):
+            if hi > lo:
+                assert_product(out[lo:hi], a[lo:hi], b[e], sa[lo:hi], sb[e], None, gated)
+                alone = int8.gemm(a[lo:hi], b[e], sa[lo:hi], sb[e], gated=gated, out_dtype=dtype)
+                assert torch.equal(alone, out[lo:hi])
+    int8.check_status(DEV)
+
+
+def test_a_captured_fork_and_join():
+    """A product of what two streams made, one of them by a kernel that lets the next begin early: the
+    graph waits for both."""
+    g = rng_of(61)
+    x, residual = (torch.randn((300, 2048), device=DEV, generator=g) for _ in range(2))
+    w = 0.5 + torch.rand(2048, device=DEV, generator=g)
+    b, sb = int8.quantize_tokens(torch.randn((512, 2048), device=DEV, generator=g))
+    offsets = torch.tensor([0, 300], dtype=torch.int32, device=DEV)
+    side = torch.cuda.Stream(DEV)
+
+    def work():
+        here = torch.cuda.current_stream()
+        side.wait_stream(here)
+        with torch.cuda.stream(side):
+            weights, scales = int8.quantize_tokens(residual[:256])
+            scales.record_stream(here)
+            weights.record_stream(here)
+        _, q, s = int8.residual_norm(x, residual, post_weight=w, next_weight=w, quantize=True)
+        here.wait_stream(side)
+        y = int8.gemm(q, weights, s, scales, out_dtype=torch.float32)
+        return y, int8.grouped_gemm(q, b[None], s, sb[None], offsets)
+
+    work()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = work()
+    for seed in (1, 2, 3):
+        for t in (x, residual):
+            t.copy_(torch.randn(t.shape, device=DEV, generator=rng_of(seed + 10 * (t is x))))
+        graph.replay()
+        torch.cuda.synchronize()
+        _, q, s = int8.residual_norm(x, residual, post_weight=w, next_weight=w, quantize=True)
+        weights, scales = int8.quantize_tokens(residual[:256])
+        torch.cuda.synchronize()
+        assert torch.equal(out[0], int8.gemm(q, weights, s, scales, out_dtype=torch.float32))
+        assert torch.equal(out[1], int8.gemm(q, b, s, sb))
