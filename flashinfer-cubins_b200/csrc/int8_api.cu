@@ -1,5 +1,6 @@
 // Host side of the 8-bit-integer operators of include/nvfp4_b200.h: argument checks and
-// launches. Nothing here keeps state between calls, allocates, throws or synchronises.
+// launches. Nothing here allocates, throws or (but for the status call) synchronises; what is kept
+// between calls are properties of devices.
 
 #include "../../include/nvfp4_b200.h"
 

@@ -10,7 +10,7 @@
 // is that of their results, stage 32 tokens of a warp's channels and store them by one copy.
 //
 // Warps of a CTA: 0 loads (one thread issues cp.async.bulk.tensor into a ring of
-// stages of 128 k), 1 issues tcgen05.mma.kind::i8 (32 k each) into one of two accumulators in
+// stages of SUB pieces of 128 k), 1 issues tcgen05.mma.kind::i8 (32 k each) into one of two accumulators in
 // tensor memory, the others take the other accumulator out, scale and store it. CTAS = 2: a pair of CTAs
 // on neighbouring SMs works on 256 channel rows with tcgen05.mma.cta_group::2; each loads its own
 // 128 rows of B and half of the tile's tokens.
@@ -556,8 +556,8 @@ int8_tile_kernel(const __grid_constant__ Int8TileParams p) {
       const float sb = next.sb, bias = next.bias;
       sa_stage[lane] = next.sa[0];
       sa_stage[32 + lane] = next.sa[1];
-      // The next tile's scales are on their way while this tile's MMAs run and its results leave: each
-      // tile fetching its own takes 44 us for 8192 x 8192 x 256, this 39.5.
+      // The next tile's scales are on their way while this tile's MMAs run and its results leave: with
+      // each tile fetching its own 8192 x 8192 x 256 took 38.6 us, so 34.7.
       if (t + step < tiles) next = share_of(t + step);
       __syncwarp();
       if (!mbar_wait(smem_u32(&bar_acc_full[acc]), acc_phase, abort_ptr)) {

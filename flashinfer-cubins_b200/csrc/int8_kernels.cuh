@@ -604,9 +604,11 @@ __global__ void __launch_bounds__(1024) int8_quantize_long_kernel(const Quantize
 // Products and routing
 // ---------------------------------------------------------------------------
 
-// x * sigmoid(x) with the approximate exponential and reciprocal (2^-22 and 2^-23 relative): no slow
-// path where exp(-x) overflows, its reciprocal is 0 there (from x = -87.3 on, where the value is
-// below 1e-36).
+// x * sigmoid(x) with the approximate exponential and reciprocal (2^-22 and 2^-23 relative). Where x is
+// well below zero the rounding of x log2(e) and of its constant counts for more: the exponential turns
+// them into up to 1.25 |x| 2^-24 of the value, 4.5e-6 at x = -60. That is far below a rounding to 16 bits
+// and seen by FP32 results alone. No slow path where exp(-x) overflows, its reciprocal is 0 there (from
+// x = -87.3 on, where the value is below 1e-36).
 __device__ __forceinline__ float silu(float x) {
   float e, r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x * -1.4426950408889634f));
@@ -615,7 +617,7 @@ __device__ __forceinline__ float silu(float x) {
 }
 
 // Routing of pairs to unpadded groups: offsets[e] = number of pairs of the experts before e
-// (offsets[experts]: of all), and a cursor per expert that starts there.
+// (offsets[experts]: of all).
 __global__ void expert_offsets_kernel(const int* __restrict__ counts, int experts,
                                       int* __restrict__ offsets) {
   __shared__ int scan[1024];

@@ -146,7 +146,7 @@ def gemm(a: torch.Tensor, b: torch.Tensor, a_scales: torch.Tensor, b_scales: tor
     """``(a @ b.T) * a_scales[:, None] * b_scales + bias`` of INT8 codes ``a [m, k]`` and
     ``b [n, k]``, summed exactly in 32-bit integers and rounded once to ``out_dtype`` (FP16, BF16 or
     FP32). With ``gated`` ``b`` is ``[2n, k]``, gate rows before up rows, and the result
-    ``silu(gate) * up`` ``[m, n]``. ``out``: a tensor to write it to."""
+    ``silu(gate) * up`` ``[m, n]``. ``k`` and ``n`` are at least 1. ``out``: a tensor to write it to."""
     index = a.get_device()
     if torch.is_grad_enabled() and (a_scales.requires_grad or b_scales.requires_grad
                                     or (bias is not None and bias.requires_grad)
@@ -271,12 +271,15 @@ def residual_norm(x: torch.Tensor, residual: torch.Tensor | None = None, *,
         r = residual_scale * residual + gate * p
         y = r / rms(r) * next_weight            rms(v) = sqrt(mean(v ** 2) + eps)
 
+    ``residual_scale`` multiplies the residual stream; a factor of the block's output, which some models
+    have there, is a ``gate`` that holds it in every element.
+
     Returns ``(r, y, scales)``: ``r`` in the residual's type, ``y`` (of the unrounded ``r``) in
     ``out_dtype`` (default: the residual's type) or, with ``quantize``, as INT8 codes with their
     ``scales``; what is not made is None. ``gate`` is ``[hidden]`` or ``[gates, hidden]``, each row
-    for ``tokens / gates`` consecutive tokens. Weights and gate are FP32, ``eps`` is at least 1e-77. Without a residual
-    only ``y = x / rms(x) * next_weight`` is made. ``residual_out`` (may be ``residual`` itself) and ``out``
-    (``y``, or codes and scales) are tensors to write to."""
+    for ``tokens / gates`` consecutive tokens. Weights and gate are FP32, ``eps`` is at least 1e-77.
+    Without a residual only ``y = x / rms(x) * next_weight`` is made. ``residual_out`` (may be
+    ``residual`` itself) and ``out`` (``y``, or codes and scales) are tensors to write to."""
     index, device = x.get_device(), x.device
     if torch.is_grad_enabled() and (
             x.requires_grad or (residual is not None and residual.requires_grad)

@@ -525,8 +525,8 @@ class Int8MoELayer:
     expert's value may pass the largest FP16 number while the token's is ordinary.
 
     The experts' rows follow one another without padding and their offsets stay on the device
-    (``nvfp4_moe_offsets``), so a forward is a fixed sequence of nine launches that reads nothing
-    back. Its buffers belong to the forward: calls on several streams and captured graphs share
+    (``nvfp4_moe_offsets``), so a forward is a fixed sequence of eight kernels and three clears that
+    reads nothing back. Its buffers belong to the forward: calls on several streams and captured graphs share
     nothing but the weights. H is a multiple of 16 (of 8 for the combine), I of 16."""
 
     def __init__(self, w13, w13_scales, w2, w2_scales):

@@ -380,8 +380,10 @@ int nvfp4_moe_place_offsets(const void* ids, int ids_are_64bit, long long pairs,
  * D[m][n] = out((float(sum_k A[m][k] B[n][k]) * a_scales[m]) * b_scales[n] + bias[n]), the sum in
  * 32-bit integers (exact: k is at most 131071), the rest in FP32, rounded once. With `gated`, B
  * holds n gate rows and then n up rows (b_scales and bias as many) and D = silu(gate) * up.
- * A and B start and lie (lda, ldb, in bytes) 16-byte aligned and have at most 2^30 rows; k, n and
- * ldd (elements) are any. out_kind NVFP4_OUT_F16, _BF16 or _F32. m = 0 launches nothing. */
+ * A and B start and lie (lda, ldb, in bytes) 16-byte aligned and have at most 2^30 rows; k and n are
+ * any from 1 on, ldd (elements) any from n on. out_kind NVFP4_OUT_F16, _BF16 or _F32. m = 0 launches
+ * nothing. silu is within (8 + 1.25 |gate|) 2^-24 of its value, relative to it, for gates from -87 on and
+ * below 1e-35 in size before. */
 int nvfp4_int8_gemm(const void* a, long long lda, const void* b, long long ldb,
                     const float* a_scales, const float* b_scales, const float* bias, void* d,
                     long long ldd, int m, int n, int k, int out_kind, int gated, void* stream);

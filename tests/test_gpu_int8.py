@@ -1041,3 +1041,20 @@ def test_a_captured_fork_and_join():
         torch.cuda.synchronize()
         assert torch.equal(out[0], int8.gemm(q, weights, s, scales, out_dtype=torch.float32))
         assert torch.equal(out[1], int8.gemm(q, b, s, sb))
+
+
+def test_silu_over_its_whole_range():
+    """Gates from -1000 to 1000 in FP32, against the accuracy that the header states: two roundings of
+    2**-24, the exponential's and the reciprocal's 2**-22 and 2**-23, and 1.25 |gate| 2**-24 from the
+    rounding of the exponent; the product by the up value (1 here) is exact."""
+    gates = torch.cat([torch.linspace(-87, 87, 40001, device=DEV), torch.linspace(-1000, 1000, 4001, device=DEV),
+                       torch.tensor([0.0, -0.0, 1e-30, -1e-30, 1e30, -1e30], device=DEV)])
+    n = gates.numel()
+    a, b = torch.ones((1, 16), dtype=torch.int8, device=DEV), torch.zeros((2 * n, 16), dtype=torch.int8, device=DEV)
+    b[:, 0] = 1
+    y = int8.gemm(a, b, torch.ones(1, device=DEV), torch.cat([gates, torch.ones_like(gates)]), gated=True,
+                  out_dtype=torch.float32)[0].double()
+    g = gates.double()
+    want = g * torch.sigmoid(g)
+    bound = torch.where(g >= -87, want.abs() * (8 + 1.25 * g.abs()) * U, torch.full_like(g, 1e-35))
+    assert ((y - want).abs() <= bound).all()
