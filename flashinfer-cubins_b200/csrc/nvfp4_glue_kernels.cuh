@@ -292,11 +292,12 @@ __global__ void moe_place_kernel(const Id* __restrict__ ids, long long pairs, in
       // The blocks' first rows come from the host (a kernel parameter) or, when the layout
       // was made on the device, from device memory.
       const int first = device_starts != nullptr ? __ldg(device_starts + e) : starts.first_row[e];
-      row = first + atomicAdd(&cursors[e], 1);
-      if (row >= 0 && row < rows) {
+      // Unsigned: first rows that are not these ids' may lie anywhere, and their sums wrap.
+      const uint32_t place =
+          static_cast<uint32_t>(first) + static_cast<uint32_t>(atomicAdd(&cursors[e], 1));
+      if (place < static_cast<uint32_t>(rows)) {
+        row = static_cast<int>(place);
         token_of_row[row] = static_cast<int>(i / choices);
-      } else {  // first rows that are not these ids'
-        row = -1;
       }
     }
     row_of_pair[i] = row;
